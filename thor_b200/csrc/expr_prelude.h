@@ -76,42 +76,33 @@ __device__ __forceinline__ void tb_store_stream(void* dst, const tb_pack<BYTES>&
 }
 
 // ---- lean pair math -------------------------------------------------------------------------------
-// Bit-identical replacements for two cuda_fp16.hpp pair routines that dominate the instruction count
-// of 16-bit stages (h2exp, __h2div).  Same arithmetic per lane (fp32 multiply by log2(e),
-// ex2.approx.ftz.f32, one round-to-nearest conversion, the same special-input corrections; fp32
-// reciprocal-multiply with the same refinement for tiny quotients), but packed conversions and a
-// packed test for the rare refinement.  thor_b200_selfcheck_pair_math compares them with the toolkit
-// routines over every input (exp) and every input pair (div).
+// Two pair routines for fp16 stages, where the toolkit's h2exp and __h2div dominate the instruction count.  Both compute
+// the result in fp32 from one hardware approximation and round it to fp16; where that rounding is not certain to be the
+// toolkit's, they call the toolkit's routine.  thor_b200_selfcheck_pair_math compares them with it over every input
+// (exp) and every input pair (div).
 __device__ __forceinline__ __half2 tb_bits2half2(unsigned int v) {
     __half2 r;
     *reinterpret_cast<unsigned int*>(&r) = v;
     return r;
 }
-__device__ __forceinline__ __half2 tb_h2exp_core(const __half2 a) {
+// exp(x) = 2^(x log2 e).  For a result that is normal in fp16 |t| = |x log2 e| <= 16, so the rounded product is off by at most
+// 2^-21 and the rounded constant by 16 * 1.4e-8 of an exponent, and ex2.approx by 2^-22 of its result: together below 7.5e-7,
+// 13 units of the 24-bit result.  fp16 drops 13 of those bits, so the rounding is certain unless they lie within 13 units of the
+// midpoint 2^12 (0.33 % of the results) or the result is subnormal in fp16, where more bits are dropped.
+__device__ __forceinline__ __half2 tb_h2exp(const __half2 a) {
     const float2 f = __half22float2(a);
     float lo, hi;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(__fmaf_rn(f.x, __int_as_float(0x3fb8aa3b), __int_as_float(0x80000000))));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(__fmaf_rn(f.y, __int_as_float(0x3fb8aa3b), __int_as_float(0x80000000))));
-    return __floats2half2_rn(lo, hi);
-}
-__device__ __forceinline__ __half2 tb_h2exp_fix(const __half2 a, const __half2 r, unsigned int special, unsigned int ulp) {
-    return __hfma2(__heq2(a, tb_bits2half2(special)), tb_bits2half2(ulp), r);
-}
-__device__ __forceinline__ __half2 tb_h2exp(const __half2 a) {
-    __half2 r = tb_h2exp_core(a);
-    r = tb_h2exp_fix(a, r, 0x1F791F79u, 0x94009400u);
-    r = tb_h2exp_fix(a, r, 0x25CF25CFu, 0x94009400u);
-    r = tb_h2exp_fix(a, r, 0xC13BC13Bu, 0x04000400u);
-    r = tb_h2exp_fix(a, r, 0xC1EFC1EFu, 0x02000200u);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(f.x * 1.44269504f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(f.y * 1.44269504f));
+    const __half2 r = __floats2half2_rn(lo, hi);
+    const unsigned int bits = *reinterpret_cast<const unsigned int*>(&r);
+    const bool near_midpoint = ((__float_as_uint(lo) - (0x1000u - 13u)) & 0x1FFFu) <= 26u || ((__float_as_uint(hi) - (0x1000u - 13u)) & 0x1FFFu) <= 26u;
+    const bool subnormal = ((bits & 0xFFFFu) - 1u) < 0x3FFu || ((bits >> 16) - 1u) < 0x3FFu;
+    if (near_midpoint || subnormal) return h2exp(a);
     return r;
 }
-// Argument known to be <= 0 (or NaN): the two corrections for positive inputs can never fire.
-__device__ __forceinline__ __half2 tb_h2exp_nonpos(const __half2 a) {
-    __half2 r = tb_h2exp_core(a);
-    r = tb_h2exp_fix(a, r, 0xC13BC13Bu, 0x04000400u);
-    r = tb_h2exp_fix(a, r, 0xC1EFC1EFu, 0x02000200u);
-    return r;
-}
+// Argument known to be <= 0 (or NaN).
+__device__ __forceinline__ __half2 tb_h2exp_nonpos(const __half2 a) { return tb_h2exp(a); }
 // Lane-wise z < 0 ? if_negative : otherwise (false for -0 and NaN, like the comparison).
 __device__ __forceinline__ __half2 tb_h2sel_neg(const __half2 z, const __half2 if_negative, const __half2 otherwise) {
     const unsigned int m = __hlt2_mask(z, __half2half2(__ushort_as_half((unsigned short)0)));
@@ -131,9 +122,10 @@ __device__ __forceinline__ __half2 tb_h2div(const __half2 a, const __half2 b) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rx) : "f"(fb.x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ry) : "f"(fb.y));
     const __half2 v = __floats2half2_rn(rx * fa.x, ry * fa.y);
-    // the toolkit routine refines a lane whose quotient q satisfies 0 < |q| < 0x008F (as fp16 bits)
+    // A quotient of two 11-bit significands is never the midpoint of two normal fp16 numbers (midpoint * divisor would need
+    // more than the dividend's 11 bits), but it can be the midpoint of two subnormal ones, where the product's error decides.
     const unsigned int bits = *reinterpret_cast<const unsigned int*>(&v) & 0x7fff7fffu;
-    if (((bits & 0xffffu) - 1u) < 0x8Eu || ((bits >> 16) - 1u) < 0x8Eu) return __h2div(a, b);
+    if (((bits & 0xffffu) - 1u) < 0x3FFu || ((bits >> 16) - 1u) < 0x3FFu) return __h2div(a, b);
     return v;
 }
 
