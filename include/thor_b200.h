@@ -470,6 +470,99 @@ THOR_B200_API int thor_b200_rowprog_waits_expired(thor_b200_rowprog* prog, uint3
 THOR_B200_API void thor_b200_rowprog_destroy(thor_b200_rowprog* prog);
 
 /* ---------------------------------------------------------------------------------------------
+ * 8-bit activation checkpoints: what a training step keeps of an activation for its backward pass, at 8.25 bits an
+ * element.  A checkpoint of [rows, cols] values is two arrays:
+ *   codes   [rows, code_pitch] bytes, code_pitch = cols rounded up to 16 (the padding is written as zero), 16-byte aligned;
+ *   scales  [rows, scale_pitch] bytes, scale_pitch = ceil(cols / 32): one power of two per 32 neighbouring columns of a
+ *           row, stored as its exponent + 127 (e8m0); 255 stands for NaN.
+ * value = code * scale.  The scale is the smallest power of two (not below 2^-127) that brings the block's largest magnitude
+ * to at most the largest code (448 for fp8_e4m3, 57344 for fp8_e5m2, 127 for int8); x / scale is exact and is rounded once,
+ * to the nearest code, ties to even: the error is at most half a step of the code.  A block that holds an infinity or a
+ * NaN gets scale 255 and codes zero and unpacks as NaN throughout, so an overflow stays visible in the backward pass.
+ * Rows are independent: a range of rows of the two arrays is the checkpoint of that range.
+ * Tensors are [rows, cols] with neighbouring columns adjacent and `stride` elements between rows (any stride >= cols; the
+ * vectorised path needs 16-byte aligned rows and cols % 8 == 0).  rows == 0 is a no-op.  Outputs must not overlap inputs.
+ * No workspace, no allocation.  No counterpart in the reference, which keeps activations in full.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct thor_b200_checkpoint_desc {
+    int32_t dtype;      /* fp32 / fp16 / bf16: the tensor */
+    int32_t code_dtype; /* fp8_e4m3 / fp8_e5m2 / int8 */
+    uint64_t rows, cols; /* cols in [1, 2^31) */
+    int64_t stride;     /* elements between the tensor's rows (ignored for one row) */
+} thor_b200_checkpoint_desc;
+
+THOR_B200_API uint64_t thor_b200_checkpoint_code_pitch(uint64_t cols);
+THOR_B200_API uint64_t thor_b200_checkpoint_scale_pitch(uint64_t cols);
+THOR_B200_API int thor_b200_checkpoint_pack_launch(const thor_b200_checkpoint_desc* desc, const void* x, void* codes, void* scales, void* stream);
+THOR_B200_API int thor_b200_checkpoint_unpack_launch(const thor_b200_checkpoint_desc* desc, const void* codes, const void* scales, void* y, void* stream);
+
+/* Activations that write their checkpoint in the forward pass and read it in the backward pass, one kernel each:
+ *   forward   y = act(x)  or, gated, y = act(x) * gate;        codes / scales = pack(x), gate_codes / gate_scales = pack(gate)
+ *   backward  with x~, gate~ the unpacked checkpoints:          grad_input = grad_output [* gate~] * act'(x~),
+ *                                                               grad_gate  = grad_output * act(x~)
+ * gelu(x) = x * normcdf(x), swish(x) = x * sigmoid(x), as in Expression::gelu / Expression::swish.  Computed in fp32, one
+ * rounding.  x_stride / gate_stride / y_stride are the row strides of x, gate and y and, in the backward pass, of grad_input,
+ * grad_gate and grad_output: the two halves of one [rows, 2 * cols] projection and of its gradient need no copy. */
+enum { THOR_B200_ACTIVATION_GELU = 0, THOR_B200_ACTIVATION_SWISH = 1 };
+
+typedef struct thor_b200_checkpointed_activation_desc {
+    int32_t kind;       /* THOR_B200_ACTIVATION_* */
+    int32_t gated;      /* 0: y = act(x); 1: y = act(x) * gate */
+    int32_t dtype;      /* fp32 / fp16 / bf16: every tensor */
+    int32_t code_dtype; /* fp8_e4m3 / fp8_e5m2 / int8 */
+    uint64_t rows, cols;
+    int64_t x_stride, gate_stride, y_stride;
+} thor_b200_checkpointed_activation_desc;
+
+THOR_B200_API int thor_b200_checkpointed_activation_launch(const thor_b200_checkpointed_activation_desc* desc, const void* x, const void* gate, void* y,
+                                                           void* codes, void* scales, void* gate_codes, void* gate_scales, void* stream);
+THOR_B200_API int thor_b200_checkpointed_activation_backward_launch(const thor_b200_checkpointed_activation_desc* desc, const void* grad_output,
+                                                                    const void* codes, const void* scales, const void* gate_codes,
+                                                                    const void* gate_scales, void* grad_input, void* grad_gate, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * LayerNorm over the last axis, with what a training step keeps of it.
+ *   forward   h = x, or round(x + residual) when residual is given (written to `sum`, the next layer's residual stream);
+ *             mu = mean(h), rstd = 1 / sqrt(mean((h - mu)^2) + eps), xh = (h - mu) * rstd, y = xh * gamma + beta
+ *   backward  xh from h with its statistics, or from the checkpoint of xh;  w = grad_output * gamma
+ *             grad_input = rstd * (w - mean(w) - xh * mean(w * xh)) [+ grad_sum]
+ *             grad_gamma = sum over rows of grad_output * xh,   grad_beta = sum over rows of grad_output
+ * Statistics, sums and the column sums are held in fp32; every output is rounded once.  The sums have a fixed order, so
+ * results are the same on every run.  A LayerNorm written as an expression keeps its full input and is compiled per shape
+ * (thor_b200_rowprog_*); these entry points take any shape without compiling.
+ * gamma / beta may be NULL (1 / 0).  mean, rstd: fp32 [rows], each may be NULL in the forward pass; codes / scales (both or
+ * neither) receive the checkpoint of xh (code_dtype; 0 when none), which with rstd is all that the backward pass needs.
+ * In the backward pass exactly one of (x, mean) and (codes, scales) is given; grad_sum is the gradient that reaches `sum` by the
+ * residual stream, or NULL; grad_gamma / grad_beta are both given (grad_param_dtype: fp32 / fp16 / bf16; fp32 leaves the
+ * sums of a shard of the rows unrounded, for an allreduce) or both NULL.
+ * rows == 0 is a no-op, except that the column sums of no rows are zero.  Outputs must not overlap inputs.
+ * workspace: workspace_bytes() bytes, 16-byte aligned, not shared by launches that overlap in time; it carries nothing from
+ * one launch to the next.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct thor_b200_layernorm_desc {
+    int32_t dtype;            /* fp32 / fp16 / bf16: x, residual, sum, y, grad_output, grad_sum, grad_input */
+    int32_t param_dtype;      /* fp32 / fp16 / bf16: gamma, beta */
+    int32_t grad_param_dtype; /* backward: grad_gamma, grad_beta */
+    int32_t code_dtype;       /* fp8_e4m3 / fp8_e5m2 / int8, 0: no checkpoint */
+    float eps;                /* forward; >= 0 */
+    uint32_t reserved;        /* must be zero */
+    uint64_t rows, cols;      /* cols in [1, 2^31) */
+    int64_t x_stride;         /* elements between rows of x and, in the backward pass, of the saved x */
+    int64_t residual_stride;  /* of residual; backward: of grad_sum */
+    int64_t y_stride;         /* of y; backward: of grad_output.  sum and grad_input are dense. */
+} thor_b200_layernorm_desc;
+
+THOR_B200_API int thor_b200_layernorm_launch(const thor_b200_layernorm_desc* desc, const void* x, const void* residual, const void* gamma, const void* beta,
+                                             void* y, void* sum, float* mean, float* rstd, void* codes, void* scales, void* stream);
+THOR_B200_API int thor_b200_layernorm_backward_workspace_bytes(const thor_b200_layernorm_desc* desc, size_t* bytes);
+THOR_B200_API int thor_b200_layernorm_backward_launch(const thor_b200_layernorm_desc* desc, const void* grad_output, const void* x, const float* mean,
+                                                      const float* rstd, const void* codes, const void* scales, const void* gamma, const void* grad_sum,
+                                                      void* grad_input, void* grad_gamma, void* grad_beta, void* workspace, size_t workspace_bytes,
+                                                      void* stream);
+/* Kernels one backward launch issues. */
+THOR_B200_API int thor_b200_layernorm_backward_launch_count(const thor_b200_layernorm_desc* desc, int parameter_gradients);
+
+/* ---------------------------------------------------------------------------------------------
  * Full reduction for callers that cannot allocate.  It has no counterpart in the reference, whose
  * reductions always stamp a workspace first (CubReduction::stampValidated).
  *
