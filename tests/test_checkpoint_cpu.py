@@ -111,7 +111,7 @@ def test_backward_workspace_holds_two_partial_rows_per_slab_and_stays_small(rows
     size = C.c_size_t()
     native.check(lib.thor_b200_layernorm_backward_workspace_bytes(C.byref(norm_desc(rows=rows, cols=cols)), C.byref(size)))
     one = 2 * ((cols + 7) // 8 * 8) * 4
-    assert size.value >= 16 and (size.value % one == 0 or size.value == 16) and size.value <= max(one, 64 << 20)
+    assert size.value >= 16 and (size.value >= one) and size.value <= max(one, 64 << 20)
 
 
 def test_python_refusals_without_a_gpu():

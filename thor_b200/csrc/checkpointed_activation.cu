@@ -1,0 +1,217 @@
+// Activations that write the 8-bit checkpoint of their input in the forward pass and read it in the backward pass (the format stands in
+// checkpoint8.cuh): streaming kernels, each element read and written once.
+#include "checkpoint_walk.cuh"
+
+namespace tb {
+namespace {
+
+using namespace ck8;
+
+// act(x) and act'(x) of two neighbouring columns: gelu(x) = x Phi(x), swish(x) = x sigma(x), as Expression::gelu and
+// Expression::swish define them.
+//
+// sigma(x) = 1 / (1 + 2^(-x log2 e)) and sigma' x + sigma = value (1 - sigma) + sigma.
+// Phi(-|x|) = e^(-x^2/2) R(|x|), where R(a) = erfcx(a / sqrt 2) / 2 is smooth and falls from 1/2 like 0.4 / a: R is a polynomial in
+// t = 1 / (1 + p a) without a constant term, fitted here for the least relative error over 0 <= a <= 15, past which the
+// exponential is below the smallest normal number.  The form keeps the relative accuracy of the far tail, and the exponential is the one
+// that the derivative needs.  Degree 9: 2.1e-7 of the value as evaluated in fp32 (fp32 tensors); degree 6: 4.8e-6, a hundredth of
+// half a unit of fp16 (16-bit tensors), three instructions a pair less.  For fp32 the rounding of x^2 is carried into the exponent.
+// Two elements an instruction (f32x2) and one exponential and one reciprocal an element; the toolkit's erfcf and expf made the backward kernel
+// wait for the arithmetic pipes (GELU [2999, 11001] fp16: 112 us).
+template <int KIND, bool FULL>
+__device__ __forceinline__ void activation2(float2 x, float2& value, float2& slope) {
+    if constexpr (KIND == THOR_B200_ACTIVATION_SWISH) {
+        const float2 y = mul2(x, both(-1.44269504f));
+        const float2 d = add2(make_float2(exp2Approx(y.x), exp2Approx(y.y)), both(1.0f));
+        const float2 s = make_float2(reciprocalApprox(d.x), reciprocalApprox(d.y));
+        value = mul2(x, s);
+        slope = fma2(value, fma2(s, both(-1.0f), both(1.0f)), s);
+    } else {
+        const float2 a = make_float2(fabsf(x.x), fabsf(x.y));
+        const float2 u = fma2(a, both(FULL ? 0.345f : 0.31f), both(1.0f));
+        const float2 t = make_float2(reciprocalApprox(u.x), reciprocalApprox(u.y));
+        float2 r;
+        if constexpr (FULL) {
+            r = fma2(t, both(-0.027935062f), both(0.14324534f));
+            r = fma2(r, t, both(-0.26724964f));
+            r = fma2(r, t, both(0.18303713f));
+            r = fma2(r, t, both(-0.034956314f));
+            r = fma2(r, t, both(0.11076973f));
+            r = fma2(r, t, both(0.117477186f));
+            r = fma2(r, t, both(0.13799077f));
+            r = fma2(r, t, both(0.13762087f));
+        } else {
+            r = fma2(t, both(-0.0739324f), both(0.1804593f));
+            r = fma2(r, t, both(0.015735528f));
+            r = fma2(r, t, both(0.13343409f));
+            r = fma2(r, t, both(0.12044038f));
+            r = fma2(r, t, both(0.12386077f));
+        }
+        const float2 square = mul2(x, x);
+        const float2 half_log2e = both(-0.72134752f);
+        float2 y = mul2(square, half_log2e);
+        if constexpr (FULL) {  // square and its rounding error; an infinite x has no error to carry
+            const float2 lost = fma2(x, x, make_float2(-square.x, -square.y));
+            y = fma2(square, half_log2e, mul2(make_float2(a.x < 1e18f ? lost.x : 0.0f, a.y < 1e18f ? lost.y : 0.0f), half_log2e));
+        }
+        const float2 e = make_float2(exp2Approx(y.x), exp2Approx(y.y));
+        const float2 q = mul2(mul2(r, t), e);
+        const float2 phi = make_float2(x.x > 0.0f ? 1.0f - q.x : q.x, x.y > 0.0f ? 1.0f - q.y : q.y);
+        value = mul2(x, phi);
+        slope = fma2(mul2(x, both(0.39894228f)), e, phi);
+    }
+}
+
+template <class T, int KIND, bool GATED, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads) activationKernel(Rows<T> x, Rows<T> gate, T* __restrict__ y, int64_t y_stride, Writer out, Writer gate_out, Walk w) {
+    gridDependencyWait();
+    gridLaunchDependents();
+    uint64_t row;
+    uint32_t col, cols;
+    locate(w, row, col, cols);
+    Raw<T, ALIGNED> raw, raw_gate;
+    fetch16(x, row, col, cols, raw);
+    if constexpr (GATED) fetch16(gate, row, col, cols, raw_gate);
+    float2 v[8], r[8];
+    expand16(x, row, col, cols, raw, v);
+    writeRow16(out, row, col, cols, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float2 slope;
+        activation2<KIND, sizeof(T) == 4>(v[i], r[i], slope);
+    }
+    if constexpr (GATED) {
+        expand16(gate, row, col, cols, raw_gate, v);
+        writeRow16(gate_out, row, col, cols, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = mul2(r[i], v[i]);
+    }
+    const uint32_t lane = threadIdx.x % 32;
+    store16<ALIGNED>(y + row * y_stride, col, cols, r, lane > 0 && col > 0, lane < 31);
+}
+
+template <class T, int KIND, bool GATED, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads) activationBackwardKernel(Rows<T> grad, Reader in, Reader gate_in, T* __restrict__ grad_x, int64_t grad_x_stride,
+                                                                     T* __restrict__ grad_gate, int64_t grad_gate_stride, Walk w) {
+    gridDependencyWait();
+    gridLaunchDependents();
+    uint64_t row;
+    uint32_t col, cols;
+    locate(w, row, col, cols);
+    Raw<T, ALIGNED> raw;
+    RawCodes codes, gate_codes;
+    fetch16(grad, row, col, cols, raw);
+    fetchCodes(in, row, col, cols, codes);
+    if constexpr (GATED) fetchCodes(gate_in, row, col, cols, gate_codes);
+    float2 d[8], v[8], dx[8];
+    expandCodes<true>(in, col, cols, codes, v);  // columns past the row's end are not stored
+    expand16(grad, row, col, cols, raw, d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float2 value, slope;
+        activation2<KIND, sizeof(T) == 4>(v[i], value, slope);
+        dx[i] = mul2(d[i], slope);
+        d[i] = mul2(d[i], value);  // the gate's gradient
+    }
+    const uint32_t lane = threadIdx.x % 32;
+    const bool before = lane > 0 && col > 0, after = lane < 31;
+    if constexpr (GATED) {
+        store16<ALIGNED>(grad_gate + row * grad_gate_stride, col, cols, d, before, after);
+        expandCodes<true>(gate_in, col, cols, gate_codes, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dx[i] = mul2(dx[i], v[i]);
+    }
+    store16<ALIGNED>(grad_x + row * grad_x_stride, col, cols, dx, before, after);
+}
+
+int checkActivation(const char* who, const thor_b200_checkpointed_activation_desc* d) {
+    TB_REQUIRE(d != nullptr, "%s: null description", who);
+    TB_REQUIRE(d->kind == THOR_B200_ACTIVATION_GELU || d->kind == THOR_B200_ACTIVATION_SWISH, "%s: unknown activation %d", who, d->kind);
+    if (int st = checkShape(who, d->dtype, d->code_dtype, d->rows, d->cols)) return st;
+    if (int st = checkStride(who, "x", d->x_stride, d->rows, d->cols)) return st;
+    if (d->gated)
+        if (int st = checkStride(who, "gate", d->gate_stride, d->rows, d->cols)) return st;
+    return checkStride(who, "y", d->y_stride, d->rows, d->cols);
+}
+// The tensors that play x, gate and y (their gradients in the backward pass) and the checkpoints.
+int checkOperands(const char* who, const thor_b200_checkpointed_activation_desc& d, const void* x, const void* gate, const void* y, const void* codes, const void* scales,
+                  const void* gate_codes, const void* gate_scales) {
+    if (int st = checkTensor(who, x, d.dtype)) return st;
+    if (int st = checkTensor(who, y, d.dtype)) return st;
+    if (int st = checkCheckpoint(who, codes, scales)) return st;
+    if (!d.gated) return THOR_B200_OK;
+    if (int st = checkTensor(who, gate, d.dtype)) return st;
+    return checkCheckpoint(who, gate_codes, gate_scales);
+}
+int planActivation(const thor_b200_checkpointed_activation_desc& d, const void* x, const void* gate, const void* y, Walk* w, dim3* grid, bool* aligned) {
+    *aligned = d.cols % kVec == 0 && rowsAligned(x, d.x_stride, d.dtype, d.rows) && rowsAligned(y, d.y_stride, d.dtype, d.rows) &&
+               (!d.gated || rowsAligned(gate, d.gate_stride, d.dtype, d.rows));
+    const bool dense = denseRows(d.x_stride, d.rows, d.cols) && denseRows(d.y_stride, d.rows, d.cols) && (!d.gated || denseRows(d.gate_stride, d.rows, d.cols));
+    return planWalk(d.rows, d.cols, dense, w, grid);
+}
+// f(element, kind, gated, aligned) with the last three as integral constants
+template <class F>
+int byVariant(const thor_b200_checkpointed_activation_desc& d, bool aligned, F&& f) {
+    return byDtype(d.dtype, [&](auto t) {
+        return byFlag(d.kind == THOR_B200_ACTIVATION_SWISH, [&](auto swish) {
+            return byFlag(d.gated != 0, [&](auto gated) {
+                return byFlag(aligned, [&](auto a) {
+                    return f(t, std::integral_constant<int, decltype(swish)::value ? THOR_B200_ACTIVATION_SWISH : THOR_B200_ACTIVATION_GELU>{}, gated, a);
+                });
+            });
+        });
+    });
+}
+
+}  // namespace
+}  // namespace tb
+
+extern "C" {
+
+int thor_b200_checkpointed_activation_launch(const thor_b200_checkpointed_activation_desc* d, const void* x, const void* gate, void* y, void* codes, void* scales,
+                                             void* gate_codes, void* gate_scales, void* stream_v) {
+    using namespace tb;
+    using namespace tb::ck8;
+    const char* who = "checkpointed_activation";
+    if (int st = checkActivation(who, d)) return st;
+    if (d->rows == 0) return THOR_B200_OK;
+    if (int st = checkOperands(who, *d, x, gate, y, codes, scales, gate_codes, gate_scales)) return st;
+    Walk w;
+    dim3 grid;
+    bool aligned = false;
+    if (int st = planActivation(*d, x, gate, y, &w, &grid, &aligned)) return st;
+    const Writer out = writerOf(codes, scales, w.cols, d->code_dtype), gate_out = writerOf(gate_codes, gate_scales, w.cols, d->code_dtype);
+    return byVariant(*d, aligned, [&](auto t, auto kind, auto gated, auto a) {
+        using T = decltype(t);
+        TB_CUDA(launchDependent(activationKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, dim3(kThreads), 0,
+                                static_cast<cudaStream_t>(stream_v), rowsOf<T>(x, d->x_stride, d->rows, d->cols), rowsOf<T>(gate, d->gate_stride, d->rows, d->cols),
+                                static_cast<T*>(y), d->y_stride, out, gate_out, w));
+        countLaunch();
+        return static_cast<int>(THOR_B200_OK);
+    });
+}
+
+int thor_b200_checkpointed_activation_backward_launch(const thor_b200_checkpointed_activation_desc* d, const void* grad_output, const void* codes, const void* scales,
+                                                      const void* gate_codes, const void* gate_scales, void* grad_input, void* grad_gate, void* stream_v) {
+    using namespace tb;
+    using namespace tb::ck8;
+    const char* who = "checkpointed_activation_backward";
+    if (int st = checkActivation(who, d)) return st;
+    if (d->rows == 0) return THOR_B200_OK;
+    if (int st = checkOperands(who, *d, grad_input, grad_gate, grad_output, codes, scales, gate_codes, gate_scales)) return st;
+    Walk w;
+    dim3 grid;
+    bool aligned = false;
+    if (int st = planActivation(*d, grad_input, grad_gate, grad_output, &w, &grid, &aligned)) return st;
+    const Reader in = readerOf(codes, scales, w.cols, d->code_dtype), gate_in = readerOf(gate_codes, gate_scales, w.cols, d->code_dtype);
+    return byVariant(*d, aligned, [&](auto t, auto kind, auto gated, auto a) {
+        using T = decltype(t);
+        TB_CUDA(launchDependent(activationBackwardKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, dim3(kThreads), 0,
+                                static_cast<cudaStream_t>(stream_v), rowsOf<T>(grad_output, d->y_stride, d->rows, d->cols), in, gate_in, static_cast<T*>(grad_input),
+                                d->x_stride, static_cast<T*>(grad_gate), d->gate_stride, w));
+        countLaunch();
+        return static_cast<int>(THOR_B200_OK);
+    });
+}
+
+}  // extern "C"

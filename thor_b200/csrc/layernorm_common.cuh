@@ -1,0 +1,160 @@
+// What the LayerNorm kernels share: teams of threads, row sums, parameters, and the checks of the description.
+//
+// A row belongs to a team: 2, 4 .. 32 neighbouring lanes, or whole warps.  Thread t of a team holds columns 16 t .. of its row (and, in
+// kernels with several chunks a thread, 16 (t + k team) ..).  A CTA holds as many teams as fit; every team walks its own rows.
+#pragma once
+
+#include "checkpoint8.cuh"
+
+namespace tb {
+namespace ln {
+
+using namespace ck8;
+
+constexpr uint32_t kMaxThreads = 512;
+
+// Scratch of a CTA for row sums that several warps share: [slot][team][warp].
+struct Scratch {
+    float2 part[2][kMaxThreads / 64][16];
+};
+
+// Sums of two values over a team; every thread of it gets both.  Consecutive calls use different slots, so one barrier a call is enough.
+__device__ __forceinline__ float2 teamSum(float2 v, uint32_t team, uint32_t team_id, Scratch& scratch, int slot) {
+    if (team <= 32) {
+        for (uint32_t o = team / 2; o > 0; o /= 2) v = add2(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+        return v;
+    }
+    const uint32_t lane = threadIdx.x % 32, warps = team / 32, warp = threadIdx.x / 32 - team_id * warps;
+    // the lower half-warp keeps the first value, the upper half the second: five exchanges for the two sums
+    float s = lane < 16 ? v.x : v.y;
+    s += __shfl_xor_sync(0xffffffffu, lane < 16 ? v.y : v.x, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane % 16 == 0) reinterpret_cast<float*>(&scratch.part[slot][team_id][warp])[lane / 16] = s;
+    asm volatile("bar.sync %0, %1;" ::"r"(team_id + 1), "r"(team) : "memory");
+    s = lane % 16 < warps ? reinterpret_cast<const float*>(&scratch.part[slot][team_id][lane % 16])[lane / 16] : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float other = __shfl_xor_sync(0xffffffffu, s, 16);
+    return lane < 16 ? make_float2(s, other) : make_float2(other, s);
+}
+// The same for one value.
+__device__ __forceinline__ float teamSum(float v, uint32_t team, uint32_t team_id, Scratch& scratch, int slot) {
+    if (team <= 32) {
+        for (uint32_t o = team / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    const uint32_t lane = threadIdx.x % 32, warps = team / 32, warp = threadIdx.x / 32 - team_id * warps;
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) scratch.part[slot][team_id][warp].x = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(team_id + 1), "r"(team) : "memory");
+    v = lane % 16 < warps ? scratch.part[slot][team_id][lane % 16].x : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Sums over a CTA of up to 1024 threads, for the kernels that loop over long rows.
+__device__ __forceinline__ float ctaSum(float v, float* slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (threadIdx.x % 32 == 0) slot[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = threadIdx.x % 32 < blockDim.x / 32 ? slot[threadIdx.x % 32] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ float sum16(const float2 (&v)[8]) {
+    const float2 a = add2(add2(v[0], v[1]), add2(v[2], v[3])), b = add2(add2(v[4], v[5]), add2(v[6], v[7]));
+    const float2 s = add2(a, b);
+    return s.x + s.y;
+}
+
+// A parameter (gamma, beta) of `cols` values of any floating type.
+struct Param {
+    const void* p;
+    int dtype;
+    bool aligned;  // 16-byte aligned
+};
+template <class T>
+__device__ __forceinline__ void loadParamAs(const Param& q, uint32_t col, uint32_t cols, float2 (&v)[4]) {
+    const T* p = static_cast<const T*>(q.p) + col;
+    if (q.aligned && col + 8 <= cols) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            if constexpr (sizeof(T) == 4) {
+                v[2 * i] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+                v[2 * i + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+            } else {
+                v[0] = widen(u.x, T{});
+                v[1] = widen(u.y, T{});
+                v[2] = widen(u.z, T{});
+                v[3] = widen(u.w, T{});
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i].x = col + 2 * i < cols ? static_cast<float>(p[2 * i]) : 0.0f;
+            v[i].y = col + 2 * i + 1 < cols ? static_cast<float>(p[2 * i + 1]) : 0.0f;
+        }
+    }
+}
+// Eight neighbouring values, `absent` where there is no parameter.  They are read for every row anew, from L1 beside the row's stream: kept
+// in registers they would take a third of them.
+__device__ __forceinline__ void loadParam8(const Param& q, float absent, uint32_t col, uint32_t cols, float2 (&v)[4]) {
+    if (q.p == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = both(absent);
+    } else if (q.dtype == THOR_B200_FP32) {
+        loadParamAs<float>(q, col, cols, v);
+    } else if (q.dtype == THOR_B200_FP16) {
+        loadParamAs<__half>(q, col, cols, v);
+    } else {
+        loadParamAs<__nv_bfloat16>(q, col, cols, v);
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------
+inline Param paramOf(const void* p, int dtype) { return Param{p, dtype, isAligned(p, 16)}; }
+
+// Threads of a row of `chunks` chunks with `per_thread` of them each.
+inline uint32_t teamOf(uint64_t chunks, uint64_t per_thread) {
+    const uint64_t threads = (chunks + per_thread - 1) / per_thread;
+    uint32_t team = 2;
+    while (team < 32 && team < threads) team *= 2;
+    return team < threads ? static_cast<uint32_t>((threads + 31) / 32 * 32) : team;
+}
+
+inline int checkDesc(const char* who, const thor_b200_layernorm_desc* d) {
+    TB_REQUIRE(d != nullptr, "%s: null description", who);
+    TB_REQUIRE(valueDtypeOk(d->dtype), "%s: tensors must be fp32, fp16 or bf16, got %s", who, dtypeName(d->dtype));
+    TB_REQUIRE(valueDtypeOk(d->param_dtype), "%s: parameters must be fp32, fp16 or bf16, got %s", who, dtypeName(d->param_dtype));
+    TB_REQUIRE(d->code_dtype == 0 || codeDtypeOk(d->code_dtype), "%s: codes must be fp8_e4m3, fp8_e5m2 or int8, got %s", who, dtypeName(d->code_dtype));
+    TB_REQUIRE(d->reserved == 0, "%s: reserved must be zero", who);
+    TB_REQUIRE(d->cols > 0 && d->cols <= 0x7fffffffull, "%s: rows must have 1 to 2^31 - 1 columns", who);
+    TB_REQUIRE(d->rows <= 0x7fffffffull, "%s: more than 2^31 - 1 rows", who);
+    TB_REQUIRE(d->eps >= 0.0f, "%s: eps must not be negative", who);
+    return THOR_B200_OK;
+}
+inline int checkStride(const char* who, const char* what, int64_t stride, const thor_b200_layernorm_desc& d) {
+    TB_REQUIRE(d.rows <= 1 || (stride >= 0 && static_cast<uint64_t>(stride) >= d.cols), "%s: the row stride of %s is smaller than a row", who, what);
+    return THOR_B200_OK;
+}
+// A tensor that may be absent.
+inline int checkPointer(const char* who, const void* p, size_t alignment) {
+    TB_REQUIRE(isAligned(p, alignment), "%s: a tensor pointer is not aligned to its elements", who);
+    return THOR_B200_OK;
+}
+inline int checkKept(const char* who, const void* codes, const void* scales, const thor_b200_layernorm_desc& d) {
+    TB_REQUIRE((codes != nullptr || scales != nullptr) == (d.code_dtype != 0) && (codes != nullptr) == (scales != nullptr), "%s: codes and scales go with a code_dtype", who);
+    TB_REQUIRE(isAligned(codes, 16), "%s: codes must be 16-byte aligned", who);
+    return THOR_B200_OK;
+}
+
+}  // namespace ln
+}  // namespace tb
