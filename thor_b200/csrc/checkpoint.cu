@@ -15,8 +15,8 @@ __global__ void __launch_bounds__(kThreads) packKernel(Rows<T> x, Writer out, Wa
     uint32_t col, cols;
     locate(w, row, col, cols);
     float2 v[8];
-    load16<ALIGNED>(x, row, col, cols, v);
-    writeRow16(out, row, col, cols, v);
+    load16<ALIGNED>(x, x.p + row * x.stride + col, col, cols, v);
+    writeCodes(codesAt(out, row, col), scaleAt(out, row, col), out.code, col, cols, v);
 }
 
 template <class T, bool ALIGNED>
@@ -27,11 +27,11 @@ __global__ void __launch_bounds__(kThreads) unpackKernel(Reader in, T* __restric
     uint32_t col, cols;
     locate(w, row, col, cols);
     RawCodes raw;
-    fetchCodes(in, row, col, cols, raw);
+    fetchCodes(codesAt(in, row, col), scaleAt(in, row, col), col, cols, raw);
     float2 v[8];
-    expandCodes<true>(in, col, cols, raw, v);  // columns past the row's end are not stored
+    expandCodes<false>(in.code, col, cols, raw, v);  // columns past the row's end are not stored
     const uint32_t lane = threadIdx.x % 32;
-    store16<ALIGNED>(y + row * y_stride, col, cols, v, lane > 0 && col > 0, lane < 31);
+    store16<ALIGNED>(y + row * y_stride + col, col, cols, v, lane > 0 && col > 0, lane < 31);
 }
 
 }  // namespace

@@ -11,6 +11,8 @@
 // hold a block.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace tb {
@@ -232,16 +234,13 @@ __device__ __noinline__ uint4 edgeWord(const char* word, const void* begin, cons
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// Columns col .. col + 15 of a row of `cols`.
+// Columns col .. col + 15 of a row of `cols`; p points at the first of them.
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void fetch16(const Rows<T>& in, uint64_t row, uint32_t col, uint32_t cols, Raw<T, ALIGNED>& raw) {
-    const T* p = in.p + row * in.stride + col;
+__device__ __forceinline__ void fetch16(const Rows<T>& in, const T* p, uint32_t col, uint32_t cols, Raw<T, ALIGNED>& raw) {
     constexpr int words = (kRegs<T> + (ALIGNED ? 0 : 4)) / 4;
-    if (col >= cols) {
 #pragma unroll
-        for (int i = 0; i < 4 * words; ++i) raw.w[i] = 0;
-        return;
-    }
+    for (int i = 0; i < 4 * words; ++i) raw.w[i] = 0;
+    if (col >= cols) return;
     if constexpr (ALIGNED) {
 #pragma unroll
         for (int i = 0; i < words; i += 2) {
@@ -251,120 +250,154 @@ __device__ __forceinline__ void fetch16(const Rows<T>& in, uint64_t row, uint32_
             raw.w[4 * i + 4] = hi.x, raw.w[4 * i + 5] = hi.y, raw.w[4 * i + 6] = hi.z, raw.w[4 * i + 7] = hi.w;
         }
     } else {
-        const char* const last = reinterpret_cast<const char*>(p + min(16u, cols - col));
         const char* const word0 = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+        const char* const last = reinterpret_cast<const char*>(p + min(16u, cols - col));
+        if (word0 >= reinterpret_cast<const char*>(in.p) && word0 + 16 * words <= in.end) {
 #pragma unroll
-        for (int i = 0; i < words; ++i) {
-            const char* word = word0 + 16 * i;
-            uint4 q = make_uint4(0u, 0u, 0u, 0u);
-            if (word < last) {
-                if (word >= reinterpret_cast<const char*>(in.p) && word + 16 <= in.end) q = __ldg(reinterpret_cast<const uint4*>(word));  // shared with the neighbouring lane
-                else q = edgeWord<T>(word, in.p, in.end);
+            for (int i = 0; i < words; ++i) {
+                if (i + 1 < words || word0 + 16 * i < last) {
+                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(word0) + i);  // the last word is the neighbouring lane's first
+                    raw.w[4 * i] = q.x, raw.w[4 * i + 1] = q.y, raw.w[4 * i + 2] = q.z, raw.w[4 * i + 3] = q.w;
+                }
             }
-            raw.w[4 * i] = q.x, raw.w[4 * i + 1] = q.y, raw.w[4 * i + 2] = q.z, raw.w[4 * i + 3] = q.w;
+        } else {  // at the tensor's first or last byte
+#pragma unroll
+            for (int i = 0; i < words; ++i) {
+                if (word0 + 16 * i < last) {
+                    const uint4 q = edgeWord<T>(word0 + 16 * i, in.p, in.end);
+                    raw.w[4 * i] = q.x, raw.w[4 * i + 1] = q.y, raw.w[4 * i + 2] = q.z, raw.w[4 * i + 3] = q.w;
+                }
+            }
         }
     }
 }
 
-// r[i] = bytes 4 i + shift .. of the run of words, shift in 0 .. 16 a multiple of the element's size; MORE words follow the wanted ones.
-template <int WANTED, int MORE, bool HALVES>
-__device__ __forceinline__ void shiftWords(uint32_t (&r)[WANTED + MORE], uint32_t shift) {
-    static_assert(MORE == 4, "shift by up to four words");
+// Calls f with m as an integral constant, m elements past a 16-byte boundary.  Every row has one m, so a warp takes one or two of the branches, and
+// each of them moves whole registers (and shifts pairs by half a register where m is odd) instead of selecting by m.
+template <class T, class F>
+__device__ __forceinline__ void byOffset(const void* p, F&& f) {
+    const uint32_t m = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u) / sizeof(T);
+    switch (m) {
+        case 0: f(std::integral_constant<int, 0>{}); break;
+        case 1: f(std::integral_constant<int, 1>{}); break;
+        case 2: f(std::integral_constant<int, 2>{}); break;
+        case 3: f(std::integral_constant<int, 3>{}); break;
+        default:
+            if constexpr (sizeof(T) == 2) {
+                switch (m) {
+                    case 4: f(std::integral_constant<int, 4>{}); break;
+                    case 5: f(std::integral_constant<int, 5>{}); break;
+                    case 6: f(std::integral_constant<int, 6>{}); break;
+                    default: f(std::integral_constant<int, 7>{});
+                }
+            }
+    }
+}
+// 32-bit word that starts at element `e` of a run of words
+template <class T, int N>
+__device__ __forceinline__ uint32_t wordAt(const uint32_t (&r)[N], int e) {
+    if constexpr (sizeof(T) == 4) return r[e];
+    else return e % 2 == 0 ? r[e / 2] : __funnelshift_r(r[e / 2], r[e / 2 + 1], 16);
+}
+
+// Zeroes the columns past the row's end.
+__device__ __forceinline__ void cutRow(uint32_t col, uint32_t cols, float2 (&v)[8]) {
+    if (col + 16 > cols) {
 #pragma unroll
-    for (int i = 0; i < WANTED; ++i) r[i] = shift & 16 ? r[i + 4] : r[i];  // then nothing else is set
-#pragma unroll
-    for (int i = 0; i < WANTED + 2; ++i) r[i] = shift & 8 ? r[i + 2] : r[i];
-#pragma unroll
-    for (int i = 0; i < WANTED + 1; ++i) r[i] = shift & 4 ? r[i + 1] : r[i];
-    if constexpr (HALVES) {
-#pragma unroll
-        for (int i = 0; i < WANTED; ++i) r[i] = __funnelshift_r(r[i], r[i + 1], (shift & 2) * 8);
+        for (int i = 0; i < 8; ++i) {
+            if (col + 2 * i >= cols) v[i].x = 0.0f;
+            if (col + 2 * i + 1 >= cols) v[i].y = 0.0f;
+        }
     }
 }
 
-// The sixteen values; zero past the row's end.
+// The sixteen values that fetch16 of the same arguments has loaded; zero past the row's end.
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void expand16(const Rows<T>& in, uint64_t row, uint32_t col, uint32_t cols, const Raw<T, ALIGNED>& raw, float2 (&v)[8]) {
+__device__ __forceinline__ void expand16(const T* p, uint32_t col, uint32_t cols, const Raw<T, ALIGNED>& raw, float2 (&v)[8]) {
     if constexpr (ALIGNED) {
         widen16<T>(raw.w, v);
     } else {
-        uint32_t r[kRegs<T> + 4], w[kRegs<T>];
+        uint32_t w[kRegs<T>];
+        byOffset<T>(p, [&](auto m) {
 #pragma unroll
-        for (int i = 0; i < kRegs<T> + 4; ++i) r[i] = raw.w[i];
-        shiftWords<kRegs<T>, 4, sizeof(T) == 2>(r, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(in.p + row * in.stride + col)) & 15u);
-#pragma unroll
-        for (int i = 0; i < kRegs<T>; ++i) w[i] = r[i];
+            for (int i = 0; i < kRegs<T>; ++i) w[i] = wordAt<T>(raw.w, decltype(m)::value + i * static_cast<int>(4 / sizeof(T)));
+        });
         widen16<T>(w, v);
-        if (col + 16 > cols) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (col + 2 * i >= cols) v[i].x = 0.0f;
-                if (col + 2 * i + 1 >= cols) v[i].y = 0.0f;
-            }
-        }
+        cutRow(col, cols, v);
     }
 }
 template <bool ALIGNED, class T>
-__device__ __forceinline__ void load16(const Rows<T>& in, uint64_t row, uint32_t col, uint32_t cols, float2 (&v)[8]) {
+__device__ __forceinline__ void load16(const Rows<T>& in, const T* p, uint32_t col, uint32_t cols, float2 (&v)[8]) {
     Raw<T, ALIGNED> raw;
-    fetch16(in, row, col, cols, raw);
-    expand16(in, row, col, cols, raw, v);
+    fetch16(in, p, col, cols, raw);
+    expand16(p, col, cols, raw, v);
 }
 
-// Writes sixteen values to columns col .. of the row that starts at `row`; a lane with cols = 0 writes nothing.  All 32 lanes call it.
+// Writes sixteen values to columns col .. of a row of `cols`, from p on; a lane with cols = 0 writes nothing.  All 32 lanes call it.
 // Not ALIGNED: a lane writes the 16-byte words that start in its range, the first of them with the last elements of the lane before
-// it; `before` / `after`: that lane / the lane behind holds the sixteen columns before / behind these.  Words that reach over the row's ends or
-// over a missing neighbour are written element by element.
+// it; `before` / `after`: that lane / the lane behind holds the sixteen columns before / behind these.  Where a neighbour is missing its
+// part is left out or written in 4- and 2-byte pieces, and words that reach over the row's end are written element by element.
 template <bool ALIGNED, class T>
-__device__ __forceinline__ void store16(T* row, uint32_t col, uint32_t cols, const float2 (&v)[8], bool before, bool after) {
+__device__ __forceinline__ void store16(T* p, uint32_t col, uint32_t cols, const float2 (&v)[8], bool before, bool after) {
+    constexpr int N = kRegs<T>;
+    uint32_t own[N];
+    narrow16<T>(v, own);
     if constexpr (ALIGNED) {
-        uint32_t w[kRegs<T>];
-        narrow16<T>(v, w);
         if (col >= cols) return;
 #pragma unroll
-        for (int i = 0; i < kRegs<T>; i += 8)
-            asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(row + col) + 4 * i), "r"(w[i]), "r"(w[i + 1]),
-                         "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+        for (int i = 0; i < N; i += 8)
+            asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(p) + 4 * i), "r"(own[i]), "r"(own[i + 1]),
+                         "r"(own[i + 2]), "r"(own[i + 3]), "r"(own[i + 4]), "r"(own[i + 5]), "r"(own[i + 6]), "r"(own[i + 7])
                          : "memory");
     } else {
-        constexpr int N = kRegs<T>, E = 16 / sizeof(T);
-        uint32_t own[N], r[N + 4];
-        narrow16<T>(v, own);
+        constexpr int E = 16 / sizeof(T), PER = 4 / sizeof(T);  // elements of a 16-byte word and of a register
+        uint32_t run[4 + N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = __shfl_up_sync(0xffffffffu, own[N - 4 + i], 1);
+        for (int i = 0; i < 4; ++i) run[i] = __shfl_up_sync(0xffffffffu, own[N - 4 + i], 1);
 #pragma unroll
-        for (int i = 0; i < N; ++i) r[4 + i] = own[i];
+        for (int i = 0; i < N; ++i) run[4 + i] = own[i];
         if (col >= cols) return;
-        T* const p = row + col;
-        const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;  // bytes past a 16-byte boundary
-        shiftWords<N, 4, sizeof(T) == 2>(r, 16 - odd);
-        const int m = static_cast<int>(odd / sizeof(T));  // elements of the first word that belong to the lane before
         const int left = static_cast<int>(min(cols - col, 1u << 20));  // elements up to the row's end
-        T* const word0 = p - m;
+        byOffset<T>(p, [&](auto offset) {
+            constexpr int m = decltype(offset)::value;  // elements of the first word that belong to the lane before
+            auto element = [&](int e, uint32_t w) {     // e counted from p; the element is the low part of w
+                if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[e] = w;
+                else reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(w);
+            };
 #pragma unroll
-        for (int k = 0; k < N / 4; ++k) {
-            const int first = k * E - m;  // of the word, counted from col
-            if ((k > 0 || before || m == 0) && first + E <= left) {
-                __stcs(reinterpret_cast<uint4*>(word0 + k * E), make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]));
-            } else {
+            for (int k = 0; k < N / 4; ++k) {
+                const int first = k * E - m;  // of the word
+                uint32_t r[4];
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (first + e < left && (k > 0 || before || first + e >= 0)) {
-                        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(word0)[k * E + e] = r[4 * k + e];
-                        else reinterpret_cast<uint16_t*>(word0)[k * E + e] = static_cast<uint16_t>(r[4 * k + e / 2] >> (16 * (e % 2)));
+                for (int j = 0; j < 4; ++j) r[j] = wordAt<T>(run, E + first + j * PER);
+                if (first + E > left) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (first + e < left && (first + e >= 0 || before)) element(first + e, PER == 1 ? r[e % 4] : r[e / 2] >> (16 * (e % 2)));
+                } else if (k > 0 || m == 0 || before) {
+                    __stcs(reinterpret_cast<uint4*>(p + first), make_uint4(r[0], r[1], r[2], r[3]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j * PER >= m) *reinterpret_cast<uint32_t*>(p + first + j * PER) = r[j];
+                        else if (PER == 2 && j * PER + 1 == m) element(0, r[j] >> 16);
                     }
                 }
             }
-        }
-        if (m > 0 && left > 16 - m && !(after && left > 16)) {  // the last m elements have no lane behind to write them
+            if (m > 0 && left > 16 - m && !(after && left > 16)) {  // the last m elements have no lane behind to write them
+                if (left >= 16) {
 #pragma unroll
-            for (int e = 16 - E + 1; e < 16; ++e) {
-                if (e >= 16 - m && e < left) {
-                    if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[e] = own[e];
-                    else reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(own[e / 2] >> (16 * (e % 2)));
+                    for (int e = 16 - m; e < 16; e += PER) {
+                        if (e + PER <= 16) *reinterpret_cast<uint32_t*>(p + e) = PER == 1 ? own[e] : (e % 2 == 0 ? own[e / 2] : __funnelshift_r(own[e / 2], own[e / 2 + 1 < N ? e / 2 + 1 : e / 2], 16));
+                        else element(e, own[e / 2] >> 16);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 16 - m; e < 16; ++e)
+                        if (e < left) element(e, PER == 1 ? own[e] : own[e / 2] >> (16 * (e % 2)));
                 }
             }
-        }
+        });
     }
 }
 // Rounds sixteen values to T and back: what a reader of the stored tensor sees.
@@ -391,38 +424,35 @@ struct Reader {
     int code;
 };
 
+__device__ __forceinline__ uint8_t* codesAt(const Writer& w, uint64_t row, uint32_t col) { return w.codes + row * w.code_pitch + col; }
+__device__ __forceinline__ uint8_t* scaleAt(const Writer& w, uint64_t row, uint32_t col) { return w.scales + row * w.scale_pitch + col / kBlock; }
+
 // Sixteen columns of one row by every lane, zero past the row's end; lanes 2 k and 2 k + 1 hold one block.  All 32 lanes call it, with cols = 0
 // where a lane has no row.
-__device__ __forceinline__ void writeRow16(const Writer& w, uint64_t row, uint32_t col, uint32_t cols, const float2 (&v)[8]) {
-    const uint32_t byte = scaleByte(blockMax(maxAbs16(v)), w.code);
+__device__ __forceinline__ void writeCodes(uint8_t* codes, uint8_t* scale, int code, uint32_t col, uint32_t cols, const float2 (&v)[8]) {
+    const uint32_t byte = scaleByte(blockMax(maxAbs16(v)), code);
     if (col >= cols) return;
-    __stcs(reinterpret_cast<uint4*>(w.codes + row * w.code_pitch + col), encode16(v, byte, w.code));  // the pitch is a multiple of 16
-    if (col % kBlock == 0) w.scales[row * w.scale_pitch + col / kBlock] = static_cast<uint8_t>(byte);
+    __stcs(reinterpret_cast<uint4*>(codes), encode16(v, byte, code));  // the pitch is a multiple of 16
+    if (col % kBlock == 0) *scale = static_cast<uint8_t>(byte);
 }
 struct RawCodes {
     uint4 codes;
     uint32_t scale;
 };
-__device__ __forceinline__ void fetchCodes(const Reader& r, uint64_t row, uint32_t col, uint32_t cols, RawCodes& raw) {
+__device__ __forceinline__ const uint8_t* codesAt(const Reader& r, uint64_t row, uint32_t col) { return r.codes + row * r.code_pitch + col; }
+__device__ __forceinline__ const uint8_t* scaleAt(const Reader& r, uint64_t row, uint32_t col) { return r.scales + row * r.scale_pitch + col / kBlock; }
+__device__ __forceinline__ void fetchCodes(const uint8_t* codes, const uint8_t* scale, uint32_t col, uint32_t cols, RawCodes& raw) {
     raw.codes = make_uint4(0u, 0u, 0u, 0u);
     raw.scale = 0;
     if (col >= cols) return;
-    raw.codes = __ldcs(reinterpret_cast<const uint4*>(r.codes + row * r.code_pitch + col));
-    raw.scale = r.scales[row * r.scale_pitch + col / kBlock];
+    raw.codes = __ldcs(reinterpret_cast<const uint4*>(codes));
+    raw.scale = __ldg(scale);
 }
-// ALIGNED as for the tensors beside it; otherwise the padding behind the row's end is made zero whatever the block's scale.
-template <bool ALIGNED>
-__device__ __forceinline__ void expandCodes(const Reader& r, uint32_t col, uint32_t cols, const RawCodes& raw, float2 (&v)[8]) {
-    decode16(raw.codes, raw.scale, r.code, v);
-    if constexpr (!ALIGNED) {
-        if (col + 16 > cols) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (col + 2 * i >= cols) v[i].x = 0.0f;
-                if (col + 2 * i + 1 >= cols) v[i].y = 0.0f;
-            }
-        }
-    }
+// CUT: the padding behind the row's end is made zero whatever the block's scale.
+template <bool CUT>
+__device__ __forceinline__ void expandCodes(int code, uint32_t col, uint32_t cols, const RawCodes& raw, float2 (&v)[8]) {
+    decode16(raw.codes, raw.scale, code, v);
+    if constexpr (CUT) cutRow(col, cols, v);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------

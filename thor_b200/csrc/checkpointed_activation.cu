@@ -70,24 +70,26 @@ __global__ void __launch_bounds__(kThreads) activationKernel(Rows<T> x, Rows<T> 
     uint32_t col, cols;
     locate(w, row, col, cols);
     Raw<T, ALIGNED> raw, raw_gate;
-    fetch16(x, row, col, cols, raw);
-    if constexpr (GATED) fetch16(gate, row, col, cols, raw_gate);
+    const T* const x_at = x.p + row * x.stride + col;
+    const T* const gate_at = gate.p + row * gate.stride + col;
+    fetch16(x, x_at, col, cols, raw);
+    if constexpr (GATED) fetch16(gate, gate_at, col, cols, raw_gate);
     float2 v[8], r[8];
-    expand16(x, row, col, cols, raw, v);
-    writeRow16(out, row, col, cols, v);
+    expand16(x_at, col, cols, raw, v);
+    writeCodes(codesAt(out, row, col), scaleAt(out, row, col), out.code, col, cols, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float2 slope;
         activation2<KIND, sizeof(T) == 4>(v[i], r[i], slope);
     }
     if constexpr (GATED) {
-        expand16(gate, row, col, cols, raw_gate, v);
-        writeRow16(gate_out, row, col, cols, v);
+        expand16(gate_at, col, cols, raw_gate, v);
+        writeCodes(codesAt(gate_out, row, col), scaleAt(gate_out, row, col), gate_out.code, col, cols, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[i] = mul2(r[i], v[i]);
     }
     const uint32_t lane = threadIdx.x % 32;
-    store16<ALIGNED>(y + row * y_stride, col, cols, r, lane > 0 && col > 0, lane < 31);
+    store16<ALIGNED>(y + row * y_stride + col, col, cols, r, lane > 0 && col > 0, lane < 31);
 }
 
 template <class T, int KIND, bool GATED, bool ALIGNED>
@@ -100,12 +102,13 @@ __global__ void __launch_bounds__(kThreads) activationBackwardKernel(Rows<T> gra
     locate(w, row, col, cols);
     Raw<T, ALIGNED> raw;
     RawCodes codes, gate_codes;
-    fetch16(grad, row, col, cols, raw);
-    fetchCodes(in, row, col, cols, codes);
-    if constexpr (GATED) fetchCodes(gate_in, row, col, cols, gate_codes);
+    const T* const grad_at = grad.p + row * grad.stride + col;
+    fetch16(grad, grad_at, col, cols, raw);
+    fetchCodes(codesAt(in, row, col), scaleAt(in, row, col), col, cols, codes);
+    if constexpr (GATED) fetchCodes(codesAt(gate_in, row, col), scaleAt(gate_in, row, col), col, cols, gate_codes);
     float2 d[8], v[8], dx[8];
-    expandCodes<true>(in, col, cols, codes, v);  // columns past the row's end are not stored
-    expand16(grad, row, col, cols, raw, d);
+    expandCodes<false>(in.code, col, cols, codes, v);  // columns past the row's end are not stored
+    expand16(grad_at, col, cols, raw, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float2 value, slope;
@@ -116,12 +119,12 @@ __global__ void __launch_bounds__(kThreads) activationBackwardKernel(Rows<T> gra
     const uint32_t lane = threadIdx.x % 32;
     const bool before = lane > 0 && col > 0, after = lane < 31;
     if constexpr (GATED) {
-        store16<ALIGNED>(grad_gate + row * grad_gate_stride, col, cols, d, before, after);
-        expandCodes<true>(gate_in, col, cols, gate_codes, v);
+        store16<ALIGNED>(grad_gate + row * grad_gate_stride + col, col, cols, d, before, after);
+        expandCodes<false>(gate_in.code, col, cols, gate_codes, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dx[i] = mul2(dx[i], v[i]);
     }
-    store16<ALIGNED>(grad_x + row * grad_x_stride, col, cols, dx, before, after);
+    store16<ALIGNED>(grad_x + row * grad_x_stride + col, col, cols, dx, before, after);
 }
 
 int checkActivation(const char* who, const thor_b200_checkpointed_activation_desc* d) {

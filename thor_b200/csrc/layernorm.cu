@@ -26,25 +26,9 @@ struct Forward {
     Writer kept;  // kept.codes == nullptr: no checkpoint
     uint64_t rows;
     uint32_t cols, team;
-    float eps, count;  // count = cols
+    float eps, count, inverse;  // count = cols, inverse = 1 / cols
 };
 
-// Output and checkpoint of sixteen columns from their differences from the mean (zero past the row's end).  All 32 lanes call it.
-template <bool ALIGNED, class T>
-__device__ __forceinline__ void finish16(const Forward<T>& f, uint64_t row, uint32_t col, uint32_t cols, float2 (&v)[8], float rstd, bool before, bool after) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], both(rstd));
-    if (f.kept.codes != nullptr) writeRow16(f.kept, row, col, cols, v);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float2 p[4], q[4];
-        loadParam8(f.gamma, 1.0f, col + 8 * h, cols, p);
-        loadParam8(f.beta, 0.0f, col + 8 * h, cols, q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * h + i] = fma2(v[4 * h + i], p[i], q[i]);
-    }
-    store16<ALIGNED>(f.y + row * f.y_stride, col, cols, v, before, after);
-}
 // v - mean, zero past the row's end, and the sum of the squares
 template <bool ALIGNED>
 __device__ __forceinline__ float centre16(float2 (&v)[8], float mean, uint32_t col, uint32_t cols) {
@@ -72,37 +56,42 @@ __device__ __forceinline__ float centre16(float2 (&v)[8], float mean, uint32_t c
 
 template <class T, int CHUNKS, bool ALIGNED, bool RESIDUAL>
 __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKernel(const __grid_constant__ Forward<T> f) {
-    constexpr bool kAhead = ALIGNED && !RESIDUAL;
+    constexpr bool kAhead = ALIGNED && !RESIDUAL;  // the next row is loaded while this one is worked on
     __shared__ Scratch scratch;
+    extern __shared__ float4 planes[];  // gamma's, then beta's
     gridDependencyWait();
     gridLaunchDependents();
     const uint32_t team = f.team, team_id = threadIdx.x / team, t = threadIdx.x - team_id * team, teams = blockDim.x / team;
-    const uint32_t lane = threadIdx.x % 32;
+    const uint32_t lane = threadIdx.x % 32, chunks = CHUNKS * team;
     const bool before = team < 32 ? t > 0 : lane > 0, after = team < 32 ? t + 1 < team : lane < 31;
-    const uint64_t step = static_cast<uint64_t>(gridDim.x) * teams;
-    uint64_t row = static_cast<uint64_t>(blockIdx.x) * teams + team_id;
+    const uint32_t step = gridDim.x * teams;
+    uint32_t row = blockIdx.x * teams + team_id;
     uint32_t cols = row < f.rows ? f.cols : 0;
     Raw<T, ALIGNED> next[CHUNKS], next_residual[RESIDUAL ? CHUNKS : 1];
-    auto fetch = [&](uint64_t r, uint32_t n) {
+    auto at = [&](const Rows<T>& in, uint32_t r, int k) { return in.p + static_cast<uint64_t>(r) * in.stride + (t + k * team) * kVec; };
+    auto fetch = [&](uint32_t r, uint32_t n) {
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
-            fetch16(f.x, r, (t + k * team) * kVec, n, next[k]);
-            if constexpr (RESIDUAL) fetch16(f.residual, r, (t + k * team) * kVec, n, next_residual[k]);
+            fetch16(f.x, at(f.x, r, k), (t + k * team) * kVec, n, next[k]);
+            if constexpr (RESIDUAL) fetch16(f.residual, at(f.residual, r, k), (t + k * team) * kVec, n, next_residual[k]);
         }
     };
     if constexpr (kAhead) fetch(row, cols);
+    stageParam(f.gamma, 1.0f, planes, chunks, f.cols);
+    stageParam(f.beta, 0.0f, planes + 4 * chunks, chunks, f.cols);
+    __syncthreads();
     // the same number of turns for the whole CTA; a team without a row has cols = 0
-    for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * teams; base < f.rows; base += step, row += step) {
+    for (uint32_t base = blockIdx.x * teams; base < f.rows; base += step, row += step) {
         float2 v[CHUNKS][8];
         float s = 0.0f;
         if constexpr (!kAhead) fetch(row, cols);
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
             const uint32_t col = (t + k * team) * kVec;
-            expand16(f.x, row, col, cols, next[k], v[k]);
+            expand16(at(f.x, row, k), col, cols, next[k], v[k]);
             if constexpr (RESIDUAL) {
                 float2 r[8];
-                expand16(f.residual, row, col, cols, next_residual[k], r);
+                expand16(at(f.residual, row, k), col, cols, next_residual[k], r);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[k][i] = add2(v[k][i], r[i]);
                 roundTo16<T>(v[k]);
@@ -113,21 +102,36 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
         if constexpr (kAhead) fetch(row + step, next_cols);
         if constexpr (RESIDUAL) {
             if (f.sum != nullptr) {
+                T* const sum_at = f.sum + static_cast<uint64_t>(row) * f.cols + t * kVec;
 #pragma unroll
-                for (int k = 0; k < CHUNKS; ++k) store16<ALIGNED>(f.sum + row * f.cols, (t + k * team) * kVec, cols, v[k], before, after);
+                for (int k = 0; k < CHUNKS; ++k) store16<ALIGNED>(sum_at + k * team * kVec, (t + k * team) * kVec, cols, v[k], before, after);
             }
         }
-        const float mean = teamSum(s, team, team_id, scratch, 0) / f.count;
+        const float mean = divideBy(teamSum(s, team, team_id, scratch, 0), f.count, f.inverse);
         s = 0.0f;
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) s += centre16<ALIGNED>(v[k], mean, (t + k * team) * kVec, cols);
-        const float rstd = 1.0f / sqrtf(teamSum(s, team, team_id, scratch, 1) / f.count + f.eps);
+        const float rstd = inverseRoot(divideBy(teamSum(s, team, team_id, scratch, 1), f.count, f.inverse) + f.eps);
         if (t == 0 && cols > 0) {
             if (f.mean != nullptr) f.mean[row] = mean;
             if (f.rstd != nullptr) f.rstd[row] = rstd;
         }
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) finish16<ALIGNED>(f, row, (t + k * team) * kVec, cols, v[k], rstd, before, after);
+        for (int k = 0; k < CHUNKS; ++k) {
+            const uint32_t col = (t + k * team) * kVec;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = mul2(v[k][i], both(rstd));
+            if (f.kept.codes != nullptr) writeCodes(codesAt(f.kept, row, col), scaleAt(f.kept, row, col), f.kept.code, col, cols, v[k]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float2 g0, g1, b0, b1;
+                stagedParam(planes, chunks, t + k * team, q, g0, g1);
+                stagedParam(planes + 4 * chunks, chunks, t + k * team, q, b0, b1);
+                v[k][2 * q] = fma2(v[k][2 * q], g0, b0);
+                v[k][2 * q + 1] = fma2(v[k][2 * q + 1], g1, b1);
+            }
+            store16<ALIGNED>(f.y + static_cast<uint64_t>(row) * f.y_stride + col, col, cols, v[k], before, after);
+        }
         cols = next_cols;
     }
 }
@@ -135,10 +139,10 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
 // The row that is normalised: x, or the rounded sum.
 template <bool ALIGNED, class T>
 __device__ __forceinline__ void input16(const Forward<T>& f, uint64_t row, uint32_t col, uint32_t cols, float2 (&v)[8]) {
-    load16<ALIGNED>(f.x, row, col, cols, v);
+    load16<ALIGNED>(f.x, f.x.p + row * f.x.stride + col, col, cols, v);
     if (f.residual.p != nullptr) {
         float2 r[8];
-        load16<ALIGNED>(f.residual, row, col, cols, r);
+        load16<ALIGNED>(f.residual, f.residual.p + row * f.residual.stride + col, col, cols, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = add2(v[i], r[i]);
         roundTo16<T>(v);
@@ -160,15 +164,15 @@ __global__ void __launch_bounds__(512) forwardLoopKernel(const __grid_constant__
         const uint32_t col = static_cast<uint32_t>(at), cols = at < f.cols ? f.cols : 0;
         input16<ALIGNED>(f, row, col, cols, v);
         s += sum16(v);
-        if (f.sum != nullptr) store16<ALIGNED>(f.sum + row * f.cols, col, cols, v, lane > 0, lane < 31);
+        if (f.sum != nullptr) store16<ALIGNED>(f.sum + row * f.cols + col, col, cols, v, lane > 0, lane < 31);
     }
-    const float mean = ctaSum(s, scratch[0]) / f.count;
+    const float mean = divideBy(ctaSum(s, scratch[0]), f.count, f.inverse);
     s = 0.0f;
     for (uint64_t at = threadIdx.x * kVec; at < f.cols; at += step) {
         input16<ALIGNED>(f, row, static_cast<uint32_t>(at), f.cols, v);
         s += centre16<ALIGNED>(v, mean, static_cast<uint32_t>(at), f.cols);
     }
-    const float rstd = 1.0f / sqrtf(ctaSum(s, scratch[1]) / f.count + f.eps);
+    const float rstd = inverseRoot(divideBy(ctaSum(s, scratch[1]), f.count, f.inverse) + f.eps);
     if (threadIdx.x == 0) {
         if (f.mean != nullptr) f.mean[row] = mean;
         if (f.rstd != nullptr) f.rstd[row] = rstd;
@@ -178,7 +182,18 @@ __global__ void __launch_bounds__(512) forwardLoopKernel(const __grid_constant__
         const uint32_t col = static_cast<uint32_t>(at), cols = at < f.cols ? f.cols : 0;
         input16<ALIGNED>(f, row, col, cols, v);
         centre16<ALIGNED>(v, mean, col, cols);
-        finish16<ALIGNED>(f, row, col, cols, v, rstd, lane > 0, lane < 31);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], both(rstd));
+        if (f.kept.codes != nullptr) writeCodes(codesAt(f.kept, row, col), scaleAt(f.kept, row, col), f.kept.code, col, cols, v);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float2 p[4], q[4];
+            loadParam8(f.gamma, 1.0f, col + 8 * h, cols, p);
+            loadParam8(f.beta, 0.0f, col + 8 * h, cols, q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * h + i] = fma2(v[4 * h + i], p[i], q[i]);
+        }
+        store16<ALIGNED>(f.y + row * f.y_stride + col, col, cols, v, lane > 0, lane < 31);
     }
 }
 
@@ -202,8 +217,14 @@ int launchForward(const Forward<T>& given, bool aligned, cudaStream_t stream) {
         const dim3 grid(static_cast<unsigned>(std::min(ctas, resident))), block(f.team * teams);
         return byFlag(f.residual.p != nullptr, [&](auto residual) {
             constexpr bool R = decltype(residual)::value;
-            if (per_thread == 1) TB_CUDA(launchDependent(forwardKernel<T, 1, A, R>, grid, block, 0, stream, f));
-            else TB_CUDA(launchDependent(forwardKernel<T, 2, A, R>, grid, block, 0, stream, f));
+            const size_t shared = 8 * sizeof(float4) * per_thread * f.team;
+            if (per_thread == 1) {
+                if (int st = allowShared<&forwardKernel<T, 1, A, R>>(shared)) return st;
+                TB_CUDA(launchDependent(forwardKernel<T, 1, A, R>, grid, block, shared, stream, f));
+            } else {
+                if (int st = allowShared<&forwardKernel<T, 2, A, R>>(shared)) return st;
+                TB_CUDA(launchDependent(forwardKernel<T, 2, A, R>, grid, block, shared, stream, f));
+            }
             countLaunch();
             return static_cast<int>(THOR_B200_OK);
         });
@@ -252,6 +273,7 @@ int thor_b200_layernorm_launch(const thor_b200_layernorm_desc* d, const void* x,
         f.cols = static_cast<uint32_t>(d->cols);
         f.eps = d->eps;
         f.count = static_cast<float>(d->cols);
+        f.inverse = 1.0f / f.count;
         return launchForward<T>(f, aligned, static_cast<cudaStream_t>(stream));
     });
 }

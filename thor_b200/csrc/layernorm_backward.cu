@@ -28,7 +28,7 @@ struct Backward {
     Reader kept;
     uint64_t rows;
     uint32_t cols, team;
-    float count;       // cols
+    float count, inverse;  // cols, 1 / cols
     float* partial;    // [partial rows][2][padded], nullptr: no parameter gradients
     uint32_t padded;
     uint64_t slab_rows;  // rows of a partial row, in the kernels for long rows
@@ -38,9 +38,9 @@ struct Backward {
 template <bool KEPT, bool ALIGNED, class T>
 struct Normal {
     Raw<T, ALIGNED> raw;
-    __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetch16(b.x, row, col, cols, raw); }
+    __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetch16(b.x, b.x.p + row * b.x.stride + col, col, cols, raw); }
     __device__ __forceinline__ void expand(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols, float mean, float rstd, float2 (&n)[8]) const {
-        expand16(b.x, row, col, cols, raw, n);
+        expand16(b.x.p + row * b.x.stride + col, col, cols, raw, n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) n[i] = mul2(add2(n[i], both(-mean)), both(rstd));
     }
@@ -48,9 +48,9 @@ struct Normal {
 template <bool ALIGNED, class T>
 struct Normal<true, ALIGNED, T> {
     RawCodes raw;
-    __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetchCodes(b.kept, row, col, cols, raw); }
+    __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetchCodes(codesAt(b.kept, row, col), scaleAt(b.kept, row, col), col, cols, raw); }
     __device__ __forceinline__ void expand(const Backward<T>& b, uint64_t, uint32_t col, uint32_t cols, float, float, float2 (&n)[8]) const {
-        expandCodes<ALIGNED>(b.kept, col, cols, raw, n);
+        expandCodes<!ALIGNED>(b.kept.code, col, cols, raw, n);
     }
 };
 
@@ -77,33 +77,33 @@ __device__ __forceinline__ void finish16(const Backward<T>& b, uint64_t row, uin
     for (int i = 0; i < 8; ++i) w[i] = mul2(fma2(n[i], both(-c2), add2(w[i], both(-c1))), both(rstd));
     if (b.grad_sum.p != nullptr) {
         float2 r[8];
-        expand16(b.grad_sum, row, col, cols, stream, r);
+        expand16(b.grad_sum.p + row * b.grad_sum.stride + col, col, cols, stream, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = add2(w[i], r[i]);
     }
-    store16<ALIGNED>(b.grad_input + row * b.cols, col, cols, w, before, after);
+    store16<ALIGNED>(b.grad_input + row * b.cols + col, col, cols, w, before, after);
 }
 
 template <class T, bool KEPT, bool ALIGNED>
 __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_constant__ Backward<T> b) {
     constexpr bool kAhead = ALIGNED;  // the next row is loaded while this one is worked on
     __shared__ Scratch scratch;
-    __shared__ float gather[kVec][kMaxThreads];
+    __shared__ float4 shared[4 * kMaxThreads];  // gamma's planes, then the teams' column sums
     gridDependencyWait();
     gridLaunchDependents();
     const uint32_t team = b.team, team_id = threadIdx.x / team, t = threadIdx.x - team_id * team, teams = blockDim.x / team;
     const uint32_t lane = threadIdx.x % 32, col = t * kVec;
     const bool before = team < 32 ? t > 0 : lane > 0, after = team < 32 ? t + 1 < team : lane < 31;
-    const uint64_t step = static_cast<uint64_t>(gridDim.x) * teams;
-    uint64_t row = static_cast<uint64_t>(blockIdx.x) * teams + team_id;
+    const uint32_t step = gridDim.x * teams;
+    uint32_t row = blockIdx.x * teams + team_id;
     Raw<T, ALIGNED> grad;
     Normal<KEPT, ALIGNED, T> normal;
     float rstd = 0.0f, mean = 0.0f;
     uint32_t cols = 0;
-    auto fetch = [&](uint64_t r) {
+    auto fetch = [&](uint32_t r) {
         const bool there = r < b.rows;
         cols = there ? b.cols : 0;
-        fetch16(b.grad, r, col, cols, grad);
+        fetch16(b.grad, b.grad.p + static_cast<uint64_t>(r) * b.grad.stride + col, col, cols, grad);
         normal.fetch(b, r, col, cols);
         rstd = there ? __ldg(b.rstd + r) : 0.0f;
         if constexpr (!KEPT) mean = there ? __ldg(b.mean + r) : 0.0f;
@@ -112,31 +112,43 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < 8; ++i) dg[i] = db[i] = both(0.0f);
     if constexpr (kAhead) fetch(row);
+    stageParam(b.gamma, 1.0f, shared, team, b.cols);
+    __syncthreads();
     int slot = 0;
     // the same number of turns for the whole CTA; a team without a row has cols = 0
-    for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * teams; base < b.rows; base += step, row += step) {
+    for (uint32_t base = blockIdx.x * teams; base < b.rows; base += step, row += step) {
         if constexpr (!kAhead) fetch(row);
         float2 w[8], n[8];
-        expand16(b.grad, row, col, cols, grad, w);
+        expand16(b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col, col, cols, grad, w);
         normal.expand(b, row, col, cols, mean, rstd, n);
         const uint32_t now_cols = cols;
         const float now_rstd = rstd;
         if constexpr (kAhead) fetch(row + step);
         Raw<T, ALIGNED> stream;
-        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, row, col, now_cols, stream);
+        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + static_cast<uint64_t>(row) * b.grad_sum.stride + col, col, now_cols, stream);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             dg[i] = fma2(w[i], n[i], dg[i]);
             db[i] = add2(db[i], w[i]);
         }
         float2 s1 = both(0.0f), s2 = both(0.0f);
-        weigh16(b, col, now_cols, w, n, s1, s2);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float2 g0, g1;
+            stagedParam(shared, team, t, q, g0, g1);
+            w[2 * q] = mul2(w[2 * q], g0);
+            w[2 * q + 1] = mul2(w[2 * q + 1], g1);
+            s1 = add2(s1, add2(w[2 * q], w[2 * q + 1]));
+            s2 = fma2(w[2 * q], n[2 * q], s2);
+            s2 = fma2(w[2 * q + 1], n[2 * q + 1], s2);
+        }
         const float2 s = teamSum(make_float2(s1.x + s1.y, s2.x + s2.y), team, team_id, scratch, slot);
         slot ^= 1;
-        finish16<ALIGNED>(b, row, col, now_cols, w, n, s.x / b.count, s.y / b.count, now_rstd, stream, before, after);
+        finish16<ALIGNED>(b, row, col, now_cols, w, n, divideBy(s.x, b.count, b.inverse), divideBy(s.y, b.count, b.inverse), now_rstd, stream, before, after);
     }
     if (b.partial == nullptr) return;
     // A partial row keeps the threads' order: value i of thread t at i * team + t.
+    float* const gather = reinterpret_cast<float*>(shared);
     float* out = b.partial + static_cast<uint64_t>(blockIdx.x) * 2 * b.padded;
     for (int which = 0; which < 2; ++which, out += b.padded) {
         if (teams == 1) {
@@ -152,14 +164,14 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float2 v = which == 0 ? dg[i] : db[i];
-            gather[2 * i][threadIdx.x] = v.x;
-            gather[2 * i + 1][threadIdx.x] = v.y;
+            gather[(2 * i) * kMaxThreads + threadIdx.x] = v.x;
+            gather[(2 * i + 1) * kMaxThreads + threadIdx.x] = v.y;
         }
         __syncthreads();
         for (uint32_t j = threadIdx.x; j < kVec * team; j += blockDim.x) {
             const uint32_t i = j / team, thread = j - i * team;
             float s = 0.0f;
-            for (uint32_t k = 0; k < teams; ++k) s += gather[i][k * team + thread];
+            for (uint32_t k = 0; k < teams; ++k) s += gather[i * kMaxThreads + k * team + thread];
             out[j] = s;
         }
     }
@@ -182,23 +194,23 @@ __global__ void __launch_bounds__(512) gradInputLoopKernel(const __grid_constant
     for (uint64_t at = threadIdx.x * kVec; at < b.cols; at += step) {
         const uint32_t col = static_cast<uint32_t>(at);
         normal.fetch(b, row, col, b.cols);
-        load16<ALIGNED>(b.grad, row, col, b.cols, w);
+        load16<ALIGNED>(b.grad, b.grad.p + row * b.grad.stride + col, col, b.cols, w);
         normal.expand(b, row, col, b.cols, mean, rstd, n);
         float2 p1 = both(0.0f), p2 = both(0.0f);
         weigh16(b, col, b.cols, w, n, p1, p2);
         s1 += p1.x + p1.y;
         s2 += p2.x + p2.y;
     }
-    const float c1 = ctaSum(s1, scratch[0]) / b.count;
-    const float c2 = ctaSum(s2, scratch[1]) / b.count;
+    const float c1 = divideBy(ctaSum(s1, scratch[0]), b.count, b.inverse);
+    const float c2 = divideBy(ctaSum(s2, scratch[1]), b.count, b.inverse);
     // the trip count is the same for the whole CTA; a thread past the row's end has columns of none
     for (uint64_t base = 0; base < b.cols; base += step) {
         const uint64_t at = base + threadIdx.x * kVec;
         const uint32_t col = static_cast<uint32_t>(at), cols = at < b.cols ? b.cols : 0;
         Raw<T, ALIGNED> stream;
-        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, row, col, cols, stream);
+        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + row * b.grad_sum.stride + col, col, cols, stream);
         normal.fetch(b, row, col, cols);
-        load16<ALIGNED>(b.grad, row, col, cols, w);
+        load16<ALIGNED>(b.grad, b.grad.p + row * b.grad.stride + col, col, cols, w);
         normal.expand(b, row, col, cols, mean, rstd, n);
         float2 p1 = both(0.0f), p2 = both(0.0f);
         weigh16(b, col, cols, w, n, p1, p2);
@@ -221,7 +233,7 @@ __global__ void __launch_bounds__(256) columnSumKernel(const __grid_constant__ B
     for (uint64_t row = blockIdx.y * b.slab_rows + warp; row < end; row += 8) {
         Normal<KEPT, ALIGNED, T> normal;
         normal.fetch(b, row, col, b.cols);
-        load16<ALIGNED>(b.grad, row, col, b.cols, d);
+        load16<ALIGNED>(b.grad, b.grad.p + row * b.grad.stride + col, col, b.cols, d);
         normal.expand(b, row, col, b.cols, KEPT ? 0.0f : b.mean[row], KEPT ? 0.0f : b.rstd[row], n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -261,7 +273,7 @@ __global__ void __launch_bounds__(256) foldKernel(const float* __restrict__ part
     float s = 0.0f;
     if (j < padded) {
         const float* p = partial + static_cast<uint64_t>(blockIdx.y) * padded + j;
-#pragma unroll 8
+#pragma unroll 20
         for (uint32_t k = warp; k < partial_rows; k += 8) s += p[static_cast<uint64_t>(k) * 2 * padded];
     }
     part[warp][lane] = s;
@@ -399,6 +411,7 @@ int thor_b200_layernorm_backward_launch(const thor_b200_layernorm_desc* d, const
         b.cols = static_cast<uint32_t>(d->cols);
         b.team = p.team;
         b.count = static_cast<float>(d->cols);
+        b.inverse = 1.0f / b.count;
         b.partial = params ? static_cast<float*>(workspace) : nullptr;
         b.padded = p.padded;
         b.slab_rows = p.slab_rows;

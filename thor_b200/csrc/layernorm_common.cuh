@@ -104,8 +104,7 @@ __device__ __forceinline__ void loadParamAs(const Param& q, uint32_t col, uint32
         }
     }
 }
-// Eight neighbouring values, `absent` where there is no parameter.  They are read for every row anew, from L1 beside the row's stream: kept
-// in registers they would take a third of them.
+// Eight neighbouring values, `absent` where there is no parameter.
 __device__ __forceinline__ void loadParam8(const Param& q, float absent, uint32_t col, uint32_t cols, float2 (&v)[4]) {
     if (q.p == nullptr) {
 #pragma unroll
@@ -119,6 +118,39 @@ __device__ __forceinline__ void loadParam8(const Param& q, float absent, uint32_
     }
 }
 
+// A parameter in shared memory as fp32, for kernels that walk many rows: kept in registers it would take a quarter of them, read from global
+// memory for every row it costs a conversion and the tests of its type.  Chunk c's sixteen values lie in four planes of 16 bytes a chunk, so that
+// neighbouring threads read neighbouring words.
+__device__ __forceinline__ void stageParam(const Param& q, float absent, float4* planes, uint32_t chunks, uint32_t cols) {
+    for (uint32_t c = threadIdx.x; c < chunks; c += blockDim.x) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float2 v[4];
+            loadParam8(q, absent, c * kVec + 8 * h, cols, v);
+            planes[(2 * h) * chunks + c] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            planes[(2 * h + 1) * chunks + c] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        }
+    }
+}
+// Values 4 q .. 4 q + 3 of chunk c.
+__device__ __forceinline__ void stagedParam(const float4* planes, uint32_t chunks, uint32_t c, int q, float2& a, float2& b) {
+    const float4 v = planes[q * chunks + c];
+    a = make_float2(v.x, v.y);
+    b = make_float2(v.z, v.w);
+}
+
+// s / count, inverse = 1 / count rounded: the quotient of the product is off by its roundings, the remainder mends it.
+__device__ __forceinline__ float divideBy(float s, float count, float inverse) {
+    const float q = s * inverse;
+    return isfinite(q) ? fmaf(fmaf(-q, count, s), inverse, q) : q;
+}
+// 1 / sqrt(v): the hardware's approximation and one Newton step (its error squared is below the last place); 0, infinity and NaN as they come.
+__device__ __forceinline__ float inverseRoot(float v) {
+    float y;
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(v));
+    return v > 0.0f && isfinite(v) ? fmaf(0.5f * y, fmaf(-(v * y), y, 1.0f), y) : y;
+}
+
 // ---- host side --------------------------------------------------------------------------------------------
 inline Param paramOf(const void* p, int dtype) { return Param{p, dtype, isAligned(p, 16)}; }
 
@@ -128,6 +160,18 @@ inline uint32_t teamOf(uint64_t chunks, uint64_t per_thread) {
     uint32_t team = 2;
     while (team < 32 && team < threads) team *= 2;
     return team < threads ? static_cast<uint32_t>((threads + 31) / 32 * 32) : team;
+}
+
+// Lets a kernel use more than the default 48 KB of shared memory, once a device.
+template <auto KERNEL>
+int allowShared(size_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    TB_CUDA(cudaGetDevice(&device));
+    if (bytes <= (40u << 10) || (done.load(std::memory_order_relaxed) >> (device & 63) & 1)) return THOR_B200_OK;
+    TB_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10));
+    done.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+    return THOR_B200_OK;
 }
 
 inline int checkDesc(const char* who, const thor_b200_layernorm_desc* d) {
