@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
             if constexpr (RESIDUAL) fetch16(f.residual, at(f.residual, r, k), (t + k * team) * kVec, n, next_residual[k]);
         }
     };
-    if constexpr (kAhead) fetch(row, cols);
+    fetch(row, cols);
     stageParam(f.gamma, 1.0f, planes, chunks, f.cols);
     stageParam(f.beta, 0.0f, planes + 4 * chunks, chunks, f.cols);
     __syncthreads();
@@ -84,7 +84,6 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
     for (uint32_t base = blockIdx.x * teams; base < f.rows; base += step, row += step) {
         float2 v[CHUNKS][8];
         float s = 0.0f;
-        if constexpr (!kAhead) fetch(row, cols);
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
             const uint32_t col = (t + k * team) * kVec;
@@ -133,6 +132,7 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
             store16<ALIGNED>(f.y + static_cast<uint64_t>(row) * f.y_stride + col, col, cols, v[k], before, after);
         }
         cols = next_cols;
+        if constexpr (!kAhead) fetch(row + step, cols);
     }
 }
 

@@ -111,13 +111,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
     float2 dg[8], db[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) dg[i] = db[i] = both(0.0f);
-    if constexpr (kAhead) fetch(row);
+    fetch(row);
     stageParam(b.gamma, 1.0f, shared, team, b.cols);
     __syncthreads();
     int slot = 0;
     // the same number of turns for the whole CTA; a team without a row has cols = 0
     for (uint32_t base = blockIdx.x * teams; base < b.rows; base += step, row += step) {
-        if constexpr (!kAhead) fetch(row);
         float2 w[8], n[8];
         expand16(b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col, col, cols, grad, w);
         normal.expand(b, row, col, cols, mean, rstd, n);
@@ -145,6 +144,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
         const float2 s = teamSum(make_float2(s1.x + s1.y, s2.x + s2.y), team, team_id, scratch, slot);
         slot ^= 1;
         finish16<ALIGNED>(b, row, col, now_cols, w, n, divideBy(s.x, b.count, b.inverse), divideBy(s.y, b.count, b.inverse), now_rstd, stream, before, after);
+        if constexpr (!kAhead) fetch(row + step);
     }
     if (b.partial == nullptr) return;
     // A partial row keeps the threads' order: value i of thread t at i * team + t.
@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(256) columnSumKernel(const __grid_constant__ B
 template <class O>
 __global__ void __launch_bounds__(256) foldKernel(const float* __restrict__ partial, uint32_t padded, uint32_t cols, uint32_t team, uint32_t partial_rows,
                                                   O* __restrict__ grad_gamma, O* __restrict__ grad_beta) {
+    constexpr int kBatch = 19;
     __shared__ float part[8][33];
     gridDependencyWait();
     gridLaunchDependents();
@@ -273,8 +274,13 @@ __global__ void __launch_bounds__(256) foldKernel(const float* __restrict__ part
     float s = 0.0f;
     if (j < padded) {
         const float* p = partial + static_cast<uint64_t>(blockIdx.y) * padded + j;
-#pragma unroll 20
-        for (uint32_t k = warp; k < partial_rows; k += 8) s += p[static_cast<uint64_t>(k) * 2 * padded];
+        for (uint32_t first = warp; first < partial_rows; first += 8 * kBatch) {
+            float v[kBatch];  // all loads of a batch before the first addition: 148 partial rows are one batch
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) v[k] = first + 8 * k < partial_rows ? p[static_cast<uint64_t>(first + 8 * k) * 2 * padded] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) s += v[k];
+        }
     }
     part[warp][lane] = s;
     __syncthreads();
