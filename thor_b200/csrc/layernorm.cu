@@ -1,8 +1,9 @@
 // LayerNorm forward: residual add, statistics, output and the 8-bit checkpoint of the normalised rows in one pass.
 //
-// A row stays in registers from its load to its last store: the mean, then the mean of the squared differences from it (no cancellation),
-// then output and checkpoint.  Teams walk their rows and load the next one before they work on the current one, so the two barriers of a
-// row's sums cost latency but leave the memory busy.  A row that a CTA's registers cannot hold is read three times by a CTA that loops.
+// A row stays in registers from its load to its last store.  Every warp takes the mean of its own columns and the squared differences from
+// that; the warps' results are put together as M2 = sum of M2_w + n_w (mean_w - mean)^2, so that nothing cancels and a row costs one barrier
+// instead of two.  Teams walk their rows and load the next one before they work on the current one.  A row that a CTA's
+// registers cannot hold is read three times by a CTA that loops.
 #include <algorithm>
 
 #include "layernorm_common.cuh"
@@ -14,6 +15,10 @@ using namespace ln;
 
 constexpr uint64_t kRegisterCols = 512ull * 2 * kVec;  // longest row of a team's registers: 512 threads, two chunks each
 
+// CTAs of 512 threads an SM holds: one chunk a thread needs 64 registers, two need 128.  Up to 8192 columns one chunk is the faster form (more warps
+// to wait with): [32768, 8192] bf16 with checkpoint 230 us against 255 with two and 80 registers and 334 with two and 128.
+constexpr int residentCtas(int chunks) { return chunks == 1 ? 2 : 1; }
+
 template <class T>
 struct Forward {
     Rows<T> x, residual;
@@ -23,6 +28,7 @@ struct Forward {
     float* rstd;
     int64_t y_stride;
     Param gamma, beta;
+    bool packable;  // the parameters that are given have the tensors' type
     Writer kept;  // kept.codes == nullptr: no checkpoint
     uint64_t rows;
     uint32_t cols, team;
@@ -54,17 +60,25 @@ __device__ __forceinline__ float centre16(float2 (&v)[8], float mean, uint32_t c
     return s.x + s.y;
 }
 
-template <class T, int CHUNKS, bool ALIGNED, bool RESIDUAL>
-__global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKernel(const __grid_constant__ Forward<T> f) {
+template <class T, int CHUNKS, bool PACKED, bool ALIGNED, bool RESIDUAL>
+__global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKernel(const __grid_constant__ Forward<T> f) {
     constexpr bool kAhead = ALIGNED && !RESIDUAL;  // the next row is loaded while this one is worked on
     __shared__ Scratch scratch;
-    extern __shared__ float4 planes[];  // gamma's, then beta's
+    using Params = Staged<T, PACKED>;
+    extern __shared__ uint4 planes[];  // gamma's, then beta's
     gridDependencyWait();
     gridLaunchDependents();
     const uint32_t team = f.team, team_id = threadIdx.x / team, t = threadIdx.x - team_id * team, teams = blockDim.x / team;
     const uint32_t lane = threadIdx.x % 32, chunks = CHUNKS * team;
     const bool before = team < 32 ? t > 0 : lane > 0, after = team < 32 ? t + 1 < team : lane < 31;
     const uint32_t step = gridDim.x * teams;
+    // columns of this warp, and of the warp whose results this lane fetches
+    const uint32_t warps = team <= 32 ? 1 : team / 32, my_warp = threadIdx.x / 32 - team_id * warps;
+    const float own_count = team <= 32 ? f.count : warpColumns(my_warp, team, f.cols, CHUNKS);
+    const float its_count = lane % 16 < warps ? (team <= 32 ? f.count : warpColumns(lane % 16, team, f.cols, CHUNKS)) : 0.0f;
+    const float own_inverse = own_count > 0.0f ? 1.0f / own_count : 0.0f, its_inverse = its_count > 0.0f ? 1.0f / its_count : 0.0f;
+    const uint32_t span = team < 32 ? team : 32;  // lanes that share a row
+    int slot = 0;
     uint32_t row = blockIdx.x * teams + team_id;
     uint32_t cols = row < f.rows ? f.cols : 0;
     Raw<T, ALIGNED> next[CHUNKS], next_residual[RESIDUAL ? CHUNKS : 1];
@@ -77,8 +91,9 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
         }
     };
     fetch(row, cols);
-    stageParam(f.gamma, 1.0f, planes, chunks, f.cols);
-    stageParam(f.beta, 0.0f, planes + 4 * chunks, chunks, f.cols);
+    const uint4* const beta_planes = planes + Params::kPlanes * chunks;
+    Params::stage(f.gamma, 1.0f, planes, chunks, f.cols);
+    Params::stage(f.beta, 0.0f, planes + Params::kPlanes * chunks, chunks, f.cols);
     __syncthreads();
     // the same number of turns for the whole CTA; a team without a row has cols = 0
     for (uint32_t base = blockIdx.x * teams; base < f.rows; base += step, row += step) {
@@ -106,11 +121,24 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
                 for (int k = 0; k < CHUNKS; ++k) store16<ALIGNED>(sum_at + k * team * kVec, (t + k * team) * kVec, cols, v[k], before, after);
             }
         }
-        const float mean = divideBy(teamSum(s, team, team_id, scratch, 0), f.count, f.inverse);
-        s = 0.0f;
+        s = laneSum(s, span);
+        float mean = divideBy(s, own_count, own_inverse), m2 = 0.0f;  // of the warp's columns
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) s += centre16<ALIGNED>(v[k], mean, (t + k * team) * kVec, cols);
-        const float rstd = inverseRoot(divideBy(teamSum(s, team, team_id, scratch, 1), f.count, f.inverse) + f.eps);
+        for (int k = 0; k < CHUNKS; ++k) m2 += centre16<ALIGNED>(v[k], mean, (t + k * team) * kVec, cols);
+        m2 = laneSum(m2, span);
+        float shift = 0.0f;  // from the warp's mean to the row's
+        if (team > 32) {
+            if (lane == 0) scratch.part[slot][team_id][my_warp] = make_float2(s, m2);
+            asm volatile("bar.sync %0, %1;" ::"r"(team_id + 1), "r"(team) : "memory");
+            const float2 its = lane % 16 < warps ? scratch.part[slot][team_id][lane % 16] : make_float2(0.0f, 0.0f);
+            slot ^= 1;
+            const float row_mean = divideBy(laneSum(its.x, 16), f.count, f.inverse);
+            const float off = its_count > 0.0f ? divideBy(its.x, its_count, its_inverse) - row_mean : 0.0f;
+            m2 = laneSum(fmaf(its_count * off, off, its.y), 16);
+            shift = mean - row_mean;
+            mean = row_mean;
+        }
+        const float rstd = inverseRoot(divideBy(m2, f.count, f.inverse) + f.eps);
         if (t == 0 && cols > 0) {
             if (f.mean != nullptr) f.mean[row] = mean;
             if (f.rstd != nullptr) f.rstd[row] = rstd;
@@ -119,15 +147,16 @@ __global__ void __launch_bounds__(kMaxThreads, CHUNKS == 1 ? 2 : 1) forwardKerne
         for (int k = 0; k < CHUNKS; ++k) {
             const uint32_t col = (t + k * team) * kVec;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[k][i] = mul2(v[k][i], both(rstd));
+            for (int i = 0; i < 8; ++i) v[k][i] = mul2(add2(v[k][i], both(shift)), both(rstd));
+            if constexpr (!ALIGNED) cutRow(col, cols, v[k]);
             if (f.kept.codes != nullptr) writeCodes(codesAt(f.kept, row, col), scaleAt(f.kept, row, col), f.kept.code, col, cols, v[k]);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float2 g0, g1, b0, b1;
-                stagedParam(planes, chunks, t + k * team, q, g0, g1);
-                stagedParam(planes + 4 * chunks, chunks, t + k * team, q, b0, b1);
-                v[k][2 * q] = fma2(v[k][2 * q], g0, b0);
-                v[k][2 * q + 1] = fma2(v[k][2 * q + 1], g1, b1);
+            for (int h = 0; h < 2; ++h) {
+                float2 g[4], b[4];
+                Params::read(planes, chunks, t + k * team, h, g);
+                Params::read(beta_planes, chunks, t + k * team, h, b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[k][4 * h + i] = fma2(v[k][4 * h + i], g[i], b[i]);
             }
             store16<ALIGNED>(f.y + static_cast<uint64_t>(row) * f.y_stride + col, col, cols, v[k], before, after);
         }
@@ -210,23 +239,29 @@ int launchForward(const Forward<T>& given, bool aligned, cudaStream_t stream) {
             countLaunch();
             return static_cast<int>(THOR_B200_OK);
         }
-        const int per_thread = chunks <= 512 ? 1 : 2;
+        const int per_thread = chunks <= kMaxThreads ? 1 : 2;
         f.team = teamOf(chunks, per_thread);
-        const uint32_t teams = kMaxThreads / f.team;
-        const uint64_t ctas = (f.rows + teams - 1) / teams, resident = static_cast<uint64_t>(device->sm_count) * (per_thread == 1 ? 2 : 1) * (512 / (f.team * teams));
-        const dim3 grid(static_cast<unsigned>(std::min(ctas, resident))), block(f.team * teams);
+        const uint32_t threads = f.team * (kMaxThreads / f.team);
+        const uint64_t teams = threads / f.team, ctas = (f.rows + teams - 1) / teams;
+        const uint64_t resident = static_cast<uint64_t>(device->sm_count) * (kMaxThreads * residentCtas(per_thread) / threads);
+        const dim3 grid(static_cast<unsigned>(std::min(ctas, resident))), block(threads);
+        const bool packed = sizeof(T) == 2 && f.packable;
+        const size_t shared = (packed ? 4 : 8) * sizeof(uint4) * per_thread * f.team;
         return byFlag(f.residual.p != nullptr, [&](auto residual) {
             constexpr bool R = decltype(residual)::value;
-            const size_t shared = 8 * sizeof(float4) * per_thread * f.team;
-            if (per_thread == 1) {
-                if (int st = allowShared<&forwardKernel<T, 1, A, R>>(shared)) return st;
-                TB_CUDA(launchDependent(forwardKernel<T, 1, A, R>, grid, block, shared, stream, f));
-            } else {
-                if (int st = allowShared<&forwardKernel<T, 2, A, R>>(shared)) return st;
-                TB_CUDA(launchDependent(forwardKernel<T, 2, A, R>, grid, block, shared, stream, f));
-            }
-            countLaunch();
-            return static_cast<int>(THOR_B200_OK);
+            auto launch = [&](auto chunks_a_thread, auto in_own_type) {
+                constexpr auto kernel = &forwardKernel<T, decltype(chunks_a_thread)::value, decltype(in_own_type)::value, A, R>;
+                if (int st = allowShared<kernel>(shared)) return st;
+                TB_CUDA(launchDependent(kernel, grid, block, shared, stream, f));
+                countLaunch();
+                return static_cast<int>(THOR_B200_OK);
+            };
+            auto launchFor = [&](auto in_own_type) {
+                return per_thread == 1 ? launch(std::integral_constant<int, 1>{}, in_own_type) : launch(std::integral_constant<int, 2>{}, in_own_type);
+            };
+            if constexpr (sizeof(T) == 2)
+                if (packed) return launchFor(std::true_type{});
+            return launchFor(std::false_type{});
         });
     });
 }
@@ -268,6 +303,7 @@ int thor_b200_layernorm_launch(const thor_b200_layernorm_desc* d, const void* x,
         f.y_stride = d->y_stride;
         f.gamma = paramOf(gamma, d->param_dtype);
         f.beta = paramOf(beta, d->param_dtype);
+        f.packable = d->param_dtype == d->dtype;
         f.kept = Writer{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), codePitch(d->cols), scalePitch(d->cols), d->code_dtype};
         f.rows = d->rows;
         f.cols = static_cast<uint32_t>(d->cols);

@@ -88,7 +88,8 @@ template <class T, bool KEPT, bool ALIGNED>
 __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_constant__ Backward<T> b) {
     constexpr bool kAhead = ALIGNED;  // the next row is loaded while this one is worked on
     __shared__ Scratch scratch;
-    __shared__ float4 shared[4 * kMaxThreads];  // gamma's planes, then the teams' column sums
+    using Params = Staged<T, false>;
+    __shared__ uint4 shared[4 * kMaxThreads];  // gamma's planes, then the teams' column sums
     gridDependencyWait();
     gridLaunchDependents();
     const uint32_t team = b.team, team_id = threadIdx.x / team, t = threadIdx.x - team_id * team, teams = blockDim.x / team;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < 8; ++i) dg[i] = db[i] = both(0.0f);
     fetch(row);
-    stageParam(b.gamma, 1.0f, shared, team, b.cols);
+    Params::stage(b.gamma, 1.0f, shared, team, b.cols);
     __syncthreads();
     int slot = 0;
     // the same number of turns for the whole CTA; a team without a row has cols = 0
@@ -132,14 +133,15 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
         }
         float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float2 g0, g1;
-            stagedParam(shared, team, t, q, g0, g1);
-            w[2 * q] = mul2(w[2 * q], g0);
-            w[2 * q + 1] = mul2(w[2 * q + 1], g1);
-            s1 = add2(s1, add2(w[2 * q], w[2 * q + 1]));
-            s2 = fma2(w[2 * q], n[2 * q], s2);
-            s2 = fma2(w[2 * q + 1], n[2 * q + 1], s2);
+        for (int h = 0; h < 2; ++h) {
+            float2 g[4];
+            Params::read(shared, team, t, h, g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[4 * h + i] = mul2(w[4 * h + i], g[i]);
+                s1 = add2(s1, w[4 * h + i]);
+                s2 = fma2(w[4 * h + i], n[4 * h + i], s2);
+            }
         }
         const float2 s = teamSum(make_float2(s1.x + s1.y, s2.x + s2.y), team, team_id, scratch, slot);
         slot ^= 1;

@@ -38,21 +38,22 @@ __device__ __forceinline__ float2 teamSum(float2 v, uint32_t team, uint32_t team
     const float other = __shfl_xor_sync(0xffffffffu, s, 16);
     return lane < 16 ? make_float2(s, other) : make_float2(other, s);
 }
-// The same for one value.
-__device__ __forceinline__ float teamSum(float v, uint32_t team, uint32_t team_id, Scratch& scratch, int slot) {
-    if (team <= 32) {
-        for (uint32_t o = team / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
+// Columns that a warp of a team holds, `chunks_a_thread` runs of 512 a team apart.
+__device__ __forceinline__ float warpColumns(uint32_t warp, uint32_t team, uint32_t cols, int chunks_a_thread) {
+    uint32_t n = 0;
+    for (int k = 0; k < chunks_a_thread; ++k) {
+        const uint32_t first = (warp * 32 + k * team) * kVec;
+        n += first < cols ? min(cols - first, 32u * kVec) : 0u;
     }
-    const uint32_t lane = threadIdx.x % 32, warps = team / 32, warp = threadIdx.x / 32 - team_id * warps;
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) scratch.part[slot][team_id][warp].x = v;
-    asm volatile("bar.sync %0, %1;" ::"r"(team_id + 1), "r"(team) : "memory");
-    v = lane % 16 < warps ? scratch.part[slot][team_id][lane % 16].x : 0.0f;
-#pragma unroll
-    for (int o = 8; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    return static_cast<float>(n);
+}
+// Sum over 2, 4 .. 32 neighbouring lanes.
+__device__ __forceinline__ float laneSum(float v, uint32_t lanes) {
+    if (lanes == 32) v += __shfl_xor_sync(0xffffffffu, v, 16);
+    if (lanes >= 16) v += __shfl_xor_sync(0xffffffffu, v, 8);
+    if (lanes >= 8) v += __shfl_xor_sync(0xffffffffu, v, 4);
+    if (lanes >= 4) v += __shfl_xor_sync(0xffffffffu, v, 2);
+    return v + __shfl_xor_sync(0xffffffffu, v, 1);
 }
 
 // Sums over a CTA of up to 1024 threads, for the kernels that loop over long rows.
@@ -118,26 +119,45 @@ __device__ __forceinline__ void loadParam8(const Param& q, float absent, uint32_
     }
 }
 
-// A parameter in shared memory as fp32, for kernels that walk many rows: kept in registers it would take a quarter of them, read from global
-// memory for every row it costs a conversion and the tests of its type.  Chunk c's sixteen values lie in four planes of 16 bytes a chunk, so that
-// neighbouring threads read neighbouring words.
-__device__ __forceinline__ void stageParam(const Param& q, float absent, float4* planes, uint32_t chunks, uint32_t cols) {
-    for (uint32_t c = threadIdx.x; c < chunks; c += blockDim.x) {
+// A parameter in shared memory, for kernels that walk many rows: kept in registers it would take a quarter of them, read from global memory for
+// every row it costs the tests of its type.  As fp32, or, PACKED, in the tensors' own 16-bit type where the parameter has it, which halves
+// the words that a row reads.  Chunk c's sixteen values lie in planes of 16 bytes a chunk, so that neighbouring threads read neighbouring words.
+template <class T, bool PACKED>
+struct Staged {
+    static constexpr int kPlanes = PACKED ? 2 : 4;
+    __device__ __forceinline__ static void stage(const Param& q, float absent, uint4* planes, uint32_t chunks, uint32_t cols) {
+        for (uint32_t c = threadIdx.x; c < chunks; c += blockDim.x) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float2 v[4];
-            loadParam8(q, absent, c * kVec + 8 * h, cols, v);
-            planes[(2 * h) * chunks + c] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-            planes[(2 * h + 1) * chunks + c] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+            for (int h = 0; h < 2; ++h) {
+                float2 v[4];
+                loadParam8(q, absent, c * kVec + 8 * h, cols, v);
+                if constexpr (PACKED) {
+                    planes[h * chunks + c] = make_uint4(narrow(v[0], T{}), narrow(v[1], T{}), narrow(v[2], T{}), narrow(v[3], T{}));
+                } else {
+                    planes[(2 * h) * chunks + c] = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+                    planes[(2 * h + 1) * chunks + c] = make_uint4(__float_as_uint(v[2].x), __float_as_uint(v[2].y), __float_as_uint(v[3].x), __float_as_uint(v[3].y));
+                }
+            }
         }
     }
-}
-// Values 4 q .. 4 q + 3 of chunk c.
-__device__ __forceinline__ void stagedParam(const float4* planes, uint32_t chunks, uint32_t c, int q, float2& a, float2& b) {
-    const float4 v = planes[q * chunks + c];
-    a = make_float2(v.x, v.y);
-    b = make_float2(v.z, v.w);
-}
+    // Values 8 h .. 8 h + 7 of chunk c.
+    __device__ __forceinline__ static void read(const uint4* planes, uint32_t chunks, uint32_t c, int h, float2 (&v)[4]) {
+        if constexpr (PACKED) {
+            const uint4 a = planes[h * chunks + c];
+            v[0] = widen(a.x, T{});
+            v[1] = widen(a.y, T{});
+            v[2] = widen(a.z, T{});
+            v[3] = widen(a.w, T{});
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 a = planes[(2 * h + i) * chunks + c];
+                v[2 * i] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
+                v[2 * i + 1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+            }
+        }
+    }
+};
 
 // s / count, inverse = 1 / count rounded: the quotient of the product is off by its roundings, the remainder mends it.
 __device__ __forceinline__ float divideBy(float s, float count, float inverse) {
