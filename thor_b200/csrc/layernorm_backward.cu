@@ -28,7 +28,7 @@ struct Backward {
     Reader kept;
     uint64_t rows;
     uint32_t cols, team;
-    float count, inverse;  // cols, 1 / cols
+    float inverse;  // 1 / cols
     float* partial;    // [partial rows][2][padded], nullptr: no parameter gradients
     uint32_t padded;
     uint64_t slab_rows;  // rows of a partial row, in the kernels for long rows
@@ -73,8 +73,9 @@ __device__ __forceinline__ void weigh16(const Backward<T>& b, uint32_t col, uint
 template <bool ALIGNED, class T>
 __device__ __forceinline__ void finish16(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols, float2 (&w)[8], const float2 (&n)[8], float c1, float c2, float rstd,
                                          const Raw<T, ALIGNED>& stream, bool before, bool after) {
+    const float2 scale = both(rstd), shift = both(-rstd * c1), slope = both(-rstd * c2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = mul2(fma2(n[i], both(-c2), add2(w[i], both(-c1))), both(rstd));
+    for (int i = 0; i < 8; ++i) w[i] = fma2(n[i], slope, fma2(w[i], scale, shift));
     if (b.grad_sum.p != nullptr) {
         float2 r[8];
         expand16(b.grad_sum.p + row * b.grad_sum.stride + col, col, cols, stream, r);
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
         }
         const float2 s = teamSum(make_float2(s1.x + s1.y, s2.x + s2.y), team, team_id, scratch, slot);
         slot ^= 1;
-        finish16<ALIGNED>(b, row, col, now_cols, w, n, divideBy(s.x, b.count, b.inverse), divideBy(s.y, b.count, b.inverse), now_rstd, stream, before, after);
+        finish16<ALIGNED>(b, row, col, now_cols, w, n, s.x * b.inverse, s.y * b.inverse, now_rstd, stream, before, after);
         if constexpr (!kAhead) fetch(row + step);
     }
     if (b.partial == nullptr) return;
@@ -203,8 +204,8 @@ __global__ void __launch_bounds__(512) gradInputLoopKernel(const __grid_constant
         s1 += p1.x + p1.y;
         s2 += p2.x + p2.y;
     }
-    const float c1 = divideBy(ctaSum(s1, scratch[0]), b.count, b.inverse);
-    const float c2 = divideBy(ctaSum(s2, scratch[1]), b.count, b.inverse);
+    const float c1 = ctaSum(s1, scratch[0]) * b.inverse;
+    const float c2 = ctaSum(s2, scratch[1]) * b.inverse;
     // the trip count is the same for the whole CTA; a thread past the row's end has columns of none
     for (uint64_t base = 0; base < b.cols; base += step) {
         const uint64_t at = base + threadIdx.x * kVec;
@@ -418,8 +419,7 @@ int thor_b200_layernorm_backward_launch(const thor_b200_layernorm_desc* d, const
         b.rows = d->rows;
         b.cols = static_cast<uint32_t>(d->cols);
         b.team = p.team;
-        b.count = static_cast<float>(d->cols);
-        b.inverse = 1.0f / b.count;
+        b.inverse = 1.0f / static_cast<float>(d->cols);
         b.partial = params ? static_cast<float*>(workspace) : nullptr;
         b.padded = p.padded;
         b.slab_rows = p.slab_rows;
