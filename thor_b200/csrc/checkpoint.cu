@@ -53,15 +53,15 @@ int thor_b200_checkpoint_pack_launch(const thor_b200_checkpoint_desc* d, const v
     if (int st = checkTensor(who, x, d->dtype)) return st;
     if (int st = checkCheckpoint(who, codes, scales)) return st;
     Walk w;
-    dim3 grid;
-    if (int st = planWalk(d->rows, d->cols, denseRows(d->stride, d->rows, d->cols), &w, &grid)) return st;
+    dim3 grid, block;
+    if (int st = planWalk(d->rows, d->cols, denseRows(d->stride, d->rows, d->cols), &w, &grid, &block)) return st;
     const Writer out = writerOf(codes, scales, w.cols, d->code_dtype);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     const bool aligned = rowsAligned(x, d->stride, d->dtype, d->rows) && d->cols % kVec == 0;
     return byDtype(d->dtype, [&](auto t) {
         using T = decltype(t);
         return byFlag(aligned, [&](auto a) {
-            TB_CUDA(launchDependent(packKernel<T, decltype(a)::value>, grid, dim3(kThreads), 0, stream, rowsOf<T>(x, d->stride, d->rows, d->cols), out, w));
+            TB_CUDA(launchDependent(packKernel<T, decltype(a)::value>, grid, block, 0, stream, rowsOf<T>(x, d->stride, d->rows, d->cols), out, w));
             countLaunch();
             return static_cast<int>(THOR_B200_OK);
         });
@@ -79,15 +79,15 @@ int thor_b200_checkpoint_unpack_launch(const thor_b200_checkpoint_desc* d, const
     if (int st = checkTensor(who, y, d->dtype)) return st;
     if (int st = checkCheckpoint(who, codes, scales)) return st;
     Walk w;
-    dim3 grid;
-    if (int st = planWalk(d->rows, d->cols, denseRows(d->stride, d->rows, d->cols), &w, &grid)) return st;
+    dim3 grid, block;
+    if (int st = planWalk(d->rows, d->cols, denseRows(d->stride, d->rows, d->cols), &w, &grid, &block)) return st;
     const Reader in = readerOf(codes, scales, w.cols, d->code_dtype);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     const bool aligned = rowsAligned(y, d->stride, d->dtype, d->rows) && d->cols % kVec == 0;
     return byDtype(d->dtype, [&](auto t) {
         using T = decltype(t);
         return byFlag(aligned, [&](auto a) {
-            TB_CUDA(launchDependent(unpackKernel<T, decltype(a)::value>, grid, dim3(kThreads), 0, stream, in, static_cast<T*>(y), d->stride, w));
+            TB_CUDA(launchDependent(unpackKernel<T, decltype(a)::value>, grid, block, 0, stream, in, static_cast<T*>(y), d->stride, w));
             countLaunch();
             return static_cast<int>(THOR_B200_OK);
         });

@@ -1,7 +1,9 @@
 // How the elementwise kernels of the 8-bit checkpoints walk a [rows, cols] tensor, and the checks of their arguments.
 //
 // One chunk of sixteen columns per thread and one wave of CTAs after another: each thread has all its loads in flight before it uses the first.  A
-// tensor whose rows lie dense and whose width is a multiple of 32 is walked as one row, which saves the index division.
+// tensor whose rows lie dense and whose width is a multiple of 32 is walked as one row; other rows of at least 2048 columns get CTAs of their
+// own (blockIdx.y is the row: no index division, addresses the same for the whole CTA; Swish backward [8192, 8191] bf16 66.8 -> 59.9 us),
+// shorter ones share CTAs.
 #pragma once
 
 #include "checkpoint8.cuh"
@@ -15,9 +17,16 @@ constexpr int kThreads = 256;
 struct Walk {
     uint64_t units;
     uint32_t chunks, cols;
+    bool row_a_cta;
 };
 // This thread's chunk; cols = 0 where there is none left.
 __device__ __forceinline__ void locate(const Walk& w, uint64_t& row, uint32_t& col, uint32_t& cols) {
+    if (w.row_a_cta) {
+        row = blockIdx.y;
+        col = (blockIdx.x * blockDim.x + threadIdx.x) * kVec;
+        cols = w.cols;
+        return;
+    }
     const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
     row = 0;
     cols = unit < w.units ? w.cols : 0;
@@ -33,7 +42,7 @@ __device__ __forceinline__ void locate(const Walk& w, uint64_t& row, uint32_t& c
     }
 }
 
-inline int planWalk(uint64_t rows, uint64_t cols, bool dense, Walk* w, dim3* grid) {
+inline int planWalk(uint64_t rows, uint64_t cols, bool dense, Walk* w, dim3* grid, dim3* block) {
     if (dense && cols % kBlock == 0 && rows * cols < 0x80000000ull) {  // the checkpoint's rows are dense then, too
         cols *= rows;
         rows = 1;
@@ -41,9 +50,17 @@ inline int planWalk(uint64_t rows, uint64_t cols, bool dense, Walk* w, dim3* gri
     w->chunks = static_cast<uint32_t>(scalePitch(cols) * (kBlock / kVec));
     w->cols = static_cast<uint32_t>(cols);
     w->units = rows * w->chunks;
+    w->row_a_cta = rows > 1 && rows <= 65535 && w->chunks >= 128;
+    if (w->row_a_cta) {
+        const uint32_t segments = (w->chunks + kThreads - 1) / kThreads;
+        *grid = dim3(segments, static_cast<unsigned>(rows));
+        *block = dim3(((w->chunks + segments - 1) / segments + 31) / 32 * 32);
+        return THOR_B200_OK;
+    }
     const uint64_t ctas = (w->units + kThreads - 1) / kThreads;
     TB_REQUIRE(ctas <= 0x7FFFFFFFull, "checkpoint: too many elements for one grid");
     *grid = dim3(static_cast<unsigned>(ctas));
+    *block = dim3(kThreads);
     return THOR_B200_OK;
 }
 

@@ -55,10 +55,11 @@ __device__ __forceinline__ void activation2(float2 x, float2& value, float2& slo
             y = fma2(square, half_log2e, mul2(make_float2(a.x < 1e18f ? lost.x : 0.0f, a.y < 1e18f ? lost.y : 0.0f), half_log2e));
         }
         const float2 e = make_float2(exp2Approx(y.x), exp2Approx(y.y));
-        const float2 q = mul2(mul2(r, t), e);
+        const float2 rt = mul2(r, t);
+        const float2 q = mul2(rt, e), p = mul2(fma2(a, both(-0.39894228f), rt), e);  // Phi and slope at -|x|; those at x and -x add up to one
         const float2 phi = make_float2(x.x > 0.0f ? 1.0f - q.x : q.x, x.y > 0.0f ? 1.0f - q.y : q.y);
         value = mul2(x, phi);
-        slope = fma2(mul2(x, both(0.39894228f)), e, phi);
+        slope = make_float2(x.x > 0.0f ? 1.0f - p.x : p.x, x.y > 0.0f ? 1.0f - p.y : p.y);
     }
 }
 
@@ -146,11 +147,11 @@ int checkOperands(const char* who, const thor_b200_checkpointed_activation_desc&
     if (int st = checkTensor(who, gate, d.dtype)) return st;
     return checkCheckpoint(who, gate_codes, gate_scales);
 }
-int planActivation(const thor_b200_checkpointed_activation_desc& d, const void* x, const void* gate, const void* y, Walk* w, dim3* grid, bool* aligned) {
+int planActivation(const thor_b200_checkpointed_activation_desc& d, const void* x, const void* gate, const void* y, Walk* w, dim3* grid, dim3* block, bool* aligned) {
     *aligned = d.cols % kVec == 0 && rowsAligned(x, d.x_stride, d.dtype, d.rows) && rowsAligned(y, d.y_stride, d.dtype, d.rows) &&
                (!d.gated || rowsAligned(gate, d.gate_stride, d.dtype, d.rows));
     const bool dense = denseRows(d.x_stride, d.rows, d.cols) && denseRows(d.y_stride, d.rows, d.cols) && (!d.gated || denseRows(d.gate_stride, d.rows, d.cols));
-    return planWalk(d.rows, d.cols, dense, w, grid);
+    return planWalk(d.rows, d.cols, dense, w, grid, block);
 }
 // f(element, kind, gated, aligned) with the last three as integral constants
 template <class F>
@@ -180,13 +181,13 @@ int thor_b200_checkpointed_activation_launch(const thor_b200_checkpointed_activa
     if (d->rows == 0) return THOR_B200_OK;
     if (int st = checkOperands(who, *d, x, gate, y, codes, scales, gate_codes, gate_scales)) return st;
     Walk w;
-    dim3 grid;
+    dim3 grid, block;
     bool aligned = false;
-    if (int st = planActivation(*d, x, gate, y, &w, &grid, &aligned)) return st;
+    if (int st = planActivation(*d, x, gate, y, &w, &grid, &block, &aligned)) return st;
     const Writer out = writerOf(codes, scales, w.cols, d->code_dtype), gate_out = writerOf(gate_codes, gate_scales, w.cols, d->code_dtype);
     return byVariant(*d, aligned, [&](auto t, auto kind, auto gated, auto a) {
         using T = decltype(t);
-        TB_CUDA(launchDependent(activationKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, dim3(kThreads), 0,
+        TB_CUDA(launchDependent(activationKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, block, 0,
                                 static_cast<cudaStream_t>(stream_v), rowsOf<T>(x, d->x_stride, d->rows, d->cols), rowsOf<T>(gate, d->gate_stride, d->rows, d->cols),
                                 static_cast<T*>(y), d->y_stride, out, gate_out, w));
         countLaunch();
@@ -203,13 +204,13 @@ int thor_b200_checkpointed_activation_backward_launch(const thor_b200_checkpoint
     if (d->rows == 0) return THOR_B200_OK;
     if (int st = checkOperands(who, *d, grad_input, grad_gate, grad_output, codes, scales, gate_codes, gate_scales)) return st;
     Walk w;
-    dim3 grid;
+    dim3 grid, block;
     bool aligned = false;
-    if (int st = planActivation(*d, grad_input, grad_gate, grad_output, &w, &grid, &aligned)) return st;
+    if (int st = planActivation(*d, grad_input, grad_gate, grad_output, &w, &grid, &block, &aligned)) return st;
     const Reader in = readerOf(codes, scales, w.cols, d->code_dtype), gate_in = readerOf(gate_codes, gate_scales, w.cols, d->code_dtype);
     return byVariant(*d, aligned, [&](auto t, auto kind, auto gated, auto a) {
         using T = decltype(t);
-        TB_CUDA(launchDependent(activationBackwardKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, dim3(kThreads), 0,
+        TB_CUDA(launchDependent(activationBackwardKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, block, 0,
                                 static_cast<cudaStream_t>(stream_v), rowsOf<T>(grad_output, d->y_stride, d->rows, d->cols), in, gate_in, static_cast<T*>(grad_input),
                                 d->x_stride, static_cast<T*>(grad_gate), d->gate_stride, w));
         countLaunch();
