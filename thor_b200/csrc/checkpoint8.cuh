@@ -208,10 +208,10 @@ struct Rows {
 };
 
 // What a thread has loaded of a row.  ALIGNED: rows start on 32 bytes and have a multiple of 16 columns, so sixteen columns are whole or absent
-// and are the words themselves.  Otherwise: the 16-byte words that contain the sixteen elements, one more than they fill.
+// and are the words themselves.  Otherwise: the words of eight elements that contain the sixteen elements, one more than they fill.
 template <class T, bool ALIGNED>
 struct Raw {
-    uint32_t w[kRegs<T> + (ALIGNED ? 0 : 4)];
+    uint32_t w[ALIGNED ? kRegs<T> : kRegs<T> / 2 * 3];
 };
 
 // A word that reaches over the tensor's first or last byte, element by element.
@@ -237,60 +237,60 @@ __device__ __noinline__ uint4 edgeWord(const char* word, const void* begin, cons
 // Columns col .. col + 15 of a row of `cols`; p points at the first of them.
 template <class T, bool ALIGNED>
 __device__ __forceinline__ void fetch16(const Rows<T>& in, const T* p, uint32_t col, uint32_t cols, Raw<T, ALIGNED>& raw) {
-    constexpr int words = (kRegs<T> + (ALIGNED ? 0 : 4)) / 4;
+    constexpr int W = kRegs<T> / 2, words = ALIGNED ? 2 : 3;  // registers of a word of eight elements, words
 #pragma unroll
-    for (int i = 0; i < 4 * words; ++i) raw.w[i] = 0;
+    for (int i = 0; i < W * words; ++i) raw.w[i] = 0;
     if (col >= cols) return;
+    auto put = [&](int i, const uint4& q) { raw.w[i] = q.x, raw.w[i + 1] = q.y, raw.w[i + 2] = q.z, raw.w[i + 3] = q.w; };
     if constexpr (ALIGNED) {
 #pragma unroll
-        for (int i = 0; i < words; i += 2) {
+        for (int i = 0; i < W * words; i += 8) {
             uint4 lo, hi;
-            load256(lo, hi, reinterpret_cast<const char*>(p) + 16 * i);
-            raw.w[4 * i] = lo.x, raw.w[4 * i + 1] = lo.y, raw.w[4 * i + 2] = lo.z, raw.w[4 * i + 3] = lo.w;
-            raw.w[4 * i + 4] = hi.x, raw.w[4 * i + 5] = hi.y, raw.w[4 * i + 6] = hi.z, raw.w[4 * i + 7] = hi.w;
+            load256(lo, hi, reinterpret_cast<const uint32_t*>(p) + i);
+            put(i, lo);
+            put(i + 4, hi);
         }
     } else {
-        const char* const word0 = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+        constexpr int bytes = 4 * W;
+        const char* const word0 = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(bytes - 1));
         const char* const last = reinterpret_cast<const char*>(p + min(16u, cols - col));
-        if (word0 >= reinterpret_cast<const char*>(in.p) && word0 + 16 * words <= in.end) {
+        if (word0 >= reinterpret_cast<const char*>(in.p) && word0 + bytes * words <= in.end) {
 #pragma unroll
             for (int i = 0; i < words; ++i) {
-                if (i + 1 < words || word0 + 16 * i < last) {
-                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(word0) + i);  // the last word is the neighbouring lane's first
-                    raw.w[4 * i] = q.x, raw.w[4 * i + 1] = q.y, raw.w[4 * i + 2] = q.z, raw.w[4 * i + 3] = q.w;
+                if (i + 1 < words || word0 + bytes * i < last) {  // the last word is the neighbouring lane's first: L1 keeps it
+                    if constexpr (W == 4) {
+                        put(4 * i, __ldg(reinterpret_cast<const uint4*>(word0) + i));
+                    } else {
+                        uint4 lo, hi;
+                        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                                     : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
+                                     : "l"(word0 + bytes * i));
+                        put(8 * i, lo);
+                        put(8 * i + 4, hi);
+                    }
                 }
             }
         } else {  // at the tensor's first or last byte
 #pragma unroll
-            for (int i = 0; i < words; ++i) {
-                if (word0 + 16 * i < last) {
-                    const uint4 q = edgeWord<T>(word0 + 16 * i, in.p, in.end);
-                    raw.w[4 * i] = q.x, raw.w[4 * i + 1] = q.y, raw.w[4 * i + 2] = q.z, raw.w[4 * i + 3] = q.w;
-                }
-            }
+            for (int i = 0; i < W * words; i += 4)
+                if (word0 + 4 * i < last) put(i, edgeWord<T>(word0 + 4 * i, in.p, in.end));
         }
     }
 }
 
-// Calls f with m as an integral constant, m elements past a 16-byte boundary.  Every row has one m, so a warp takes one or two of the branches, and
-// each of them moves whole registers (and shifts pairs by half a register where m is odd) instead of selecting by m.
+// Calls f with m as an integral constant, m elements past a word of eight elements.  Every row has one m, so a warp takes one or two of the branches,
+// and each of them moves whole registers (and shifts pairs by half a register where m is odd) instead of selecting by m.
 template <class T, class F>
 __device__ __forceinline__ void byOffset(const void* p, F&& f) {
-    const uint32_t m = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u) / sizeof(T);
-    switch (m) {
+    switch ((static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) / sizeof(T)) % 8) {
         case 0: f(std::integral_constant<int, 0>{}); break;
         case 1: f(std::integral_constant<int, 1>{}); break;
         case 2: f(std::integral_constant<int, 2>{}); break;
         case 3: f(std::integral_constant<int, 3>{}); break;
-        default:
-            if constexpr (sizeof(T) == 2) {
-                switch (m) {
-                    case 4: f(std::integral_constant<int, 4>{}); break;
-                    case 5: f(std::integral_constant<int, 5>{}); break;
-                    case 6: f(std::integral_constant<int, 6>{}); break;
-                    default: f(std::integral_constant<int, 7>{});
-                }
-            }
+        case 4: f(std::integral_constant<int, 4>{}); break;
+        case 5: f(std::integral_constant<int, 5>{}); break;
+        case 6: f(std::integral_constant<int, 6>{}); break;
+        default: f(std::integral_constant<int, 7>{});
     }
 }
 // 32-bit word that starts at element `e` of a run of words
@@ -334,28 +334,32 @@ __device__ __forceinline__ void load16(const Rows<T>& in, const T* p, uint32_t c
 }
 
 // Writes sixteen values to columns col .. of a row of `cols`, from p on; a lane with cols = 0 writes nothing.  All 32 lanes call it.
-// Not ALIGNED: a lane writes the 16-byte words that start in its range, the first of them with the last elements of the lane before
-// it; `before` / `after`: that lane / the lane behind holds the sixteen columns before / behind these.  Where a neighbour is missing its
-// part is left out or written in 4- and 2-byte pieces, and words that reach over the row's end are written element by element.
+// Not ALIGNED: a lane writes the words of eight elements (32 bytes of fp32, 16 of a 16-bit type) that start in its range, the first of them with the
+// last elements of the lane before it; `before` / `after`: that lane / the lane behind holds the sixteen columns before / behind these.  Where a
+// neighbour is missing its part is left out, and what is left is written in smaller pieces; words that reach over the row's end are
+// written element by element.  (32-byte words of 16-bit types take twice the exchanges and cases: unpack [8192, 8191] bf16 46.6 us against 42;
+// 16-byte words of fp32 leave half a sector to every store: unpack [4096, 2999] 15.3 us against 9.5.)
 template <bool ALIGNED, class T>
 __device__ __forceinline__ void store16(T* p, uint32_t col, uint32_t cols, const float2 (&v)[8], bool before, bool after) {
     constexpr int N = kRegs<T>;
     uint32_t own[N];
     narrow16<T>(v, own);
+    auto wide = [](void* to, const uint32_t* w) {
+        asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                     "r"(w[7])
+                     : "memory");
+    };
     if constexpr (ALIGNED) {
         if (col >= cols) return;
 #pragma unroll
-        for (int i = 0; i < N; i += 8)
-            asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(p) + 4 * i), "r"(own[i]), "r"(own[i + 1]),
-                         "r"(own[i + 2]), "r"(own[i + 3]), "r"(own[i + 4]), "r"(own[i + 5]), "r"(own[i + 6]), "r"(own[i + 7])
-                         : "memory");
+        for (int i = 0; i < N; i += 8) wide(reinterpret_cast<uint32_t*>(p) + i, own + i);
     } else {
-        constexpr int E = 16 / sizeof(T), PER = 4 / sizeof(T);  // elements of a 16-byte word and of a register
-        uint32_t run[4 + N];
+        constexpr int E = 8, PER = 4 / sizeof(T), W = E / PER;  // elements of a word, elements of a register, registers of a word
+        uint32_t run[W + N];                                    // the lane before's last word and these
 #pragma unroll
-        for (int i = 0; i < 4; ++i) run[i] = __shfl_up_sync(0xffffffffu, own[N - 4 + i], 1);
+        for (int i = 0; i < W; ++i) run[i] = __shfl_up_sync(0xffffffffu, own[N - W + i], 1);
 #pragma unroll
-        for (int i = 0; i < N; ++i) run[4 + i] = own[i];
+        for (int i = 0; i < N; ++i) run[W + i] = own[i];
         if (col >= cols) return;
         const int left = static_cast<int>(min(cols - col, 1u << 20));  // elements up to the row's end
         byOffset<T>(p, [&](auto offset) {
@@ -365,32 +369,36 @@ __device__ __forceinline__ void store16(T* p, uint32_t col, uint32_t cols, const
                 else reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(w);
             };
 #pragma unroll
-            for (int k = 0; k < N / 4; ++k) {
+            for (int k = 0; k < N / W; ++k) {
                 const int first = k * E - m;  // of the word
-                uint32_t r[4];
+                uint32_t r[W];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] = wordAt<T>(run, E + first + j * PER);
+                for (int j = 0; j < W; ++j) r[j] = wordAt<T>(run, E + first + j * PER);
                 if (first + E > left) {
 #pragma unroll
                     for (int e = 0; e < E; ++e)
-                        if (first + e < left && (first + e >= 0 || before)) element(first + e, PER == 1 ? r[e % 4] : r[e / 2] >> (16 * (e % 2)));
+                        if (first + e < left && (first + e >= 0 || before)) element(first + e, PER == 1 ? r[e % W] : r[e / 2] >> (16 * (e % 2)));
                 } else if (k > 0 || m == 0 || before) {
-                    __stcs(reinterpret_cast<uint4*>(p + first), make_uint4(r[0], r[1], r[2], r[3]));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j * PER >= m) *reinterpret_cast<uint32_t*>(p + first + j * PER) = r[j];
-                        else if (PER == 2 && j * PER + 1 == m) element(0, r[j] >> 16);
-                    }
+                    if constexpr (W == 8) wide(p + first, r);
+                    else __stcs(reinterpret_cast<uint4*>(p + first), make_uint4(r[0], r[1], r[2], r[3]));
+                } else {  // from element m of the word on
+                    if constexpr (PER == 2 && m % 2 == 1) element(0, r[m / 2] >> 16);
+                    constexpr int one = (m + PER - 1) / PER, two = (one + 1) / 2 * 2, four = (two + 3) / 4 * 4;  // first whole register, pair, four
+                    uint32_t* const to = reinterpret_cast<uint32_t*>(p + first);
+                    if constexpr (one % 2 == 1) to[one] = r[one];
+                    if constexpr (two % 4 == 2) *reinterpret_cast<uint2*>(to + two) = make_uint2(r[two], r[two + 1]);
+                    if constexpr (four + 4 <= W) *reinterpret_cast<uint4*>(to + four) = make_uint4(r[four], r[four + 1], r[four + 2], r[four + 3]);
                 }
             }
             if (m > 0 && left > 16 - m && !(after && left > 16)) {  // the last m elements have no lane behind to write them
                 if (left >= 16) {
-#pragma unroll
-                    for (int e = 16 - m; e < 16; e += PER) {
-                        if (e + PER <= 16) *reinterpret_cast<uint32_t*>(p + e) = PER == 1 ? own[e] : (e % 2 == 0 ? own[e / 2] : __funnelshift_r(own[e / 2], own[e / 2 + 1 < N ? e / 2 + 1 : e / 2], 16));
-                        else element(e, own[e / 2] >> 16);
-                    }
+                    uint32_t* const to = reinterpret_cast<uint32_t*>(p + 16 - m);  // on a word
+                    auto reg = [&](int j) { return wordAt<T>(run, E + 16 - m + j * PER); };
+                    constexpr int n = m / PER;  // whole registers
+                    if constexpr (n >= 4) *reinterpret_cast<uint4*>(to) = make_uint4(reg(0), reg(1), reg(2), reg(3));
+                    if constexpr (n % 4 >= 2) *reinterpret_cast<uint2*>(to + n / 4 * 4) = make_uint2(reg(n / 4 * 4), reg(n / 4 * 4 + 1));
+                    if constexpr (n % 2 == 1) to[n - 1] = reg(n - 1);
+                    if constexpr (PER == 2 && m % 2 == 1) element(15, own[N - 1] >> 16);
                 } else {
 #pragma unroll
                     for (int e = 16 - m; e < 16; ++e)
