@@ -127,3 +127,33 @@ def test_python_refusals_without_a_gpu():
             make()
     with pytest.raises(ValueError):
         CheckpointedActivation(2)
+
+
+def test_pointers_off_their_elements():
+    d = _CheckpointDesc(BF16, E4M3, 4, 64, 64)
+    refused(lib.thor_b200_checkpoint_pack_launch(C.byref(d), 17, 16, 16, None), "not aligned to its elements")
+    refused(lib.thor_b200_checkpoint_unpack_launch(C.byref(d), 16, 16, 17, None), "not aligned to its elements")
+    a = _ActivationDesc(0, 1, int(DataType.fp32), E4M3, 4, 64, 64, 64, 64)
+    for at in (0, 1, 2):
+        args = [16] * 7
+        args[at] = 18
+        refused(lib.thor_b200_checkpointed_activation_launch(C.byref(a), *args, None), "not aligned to its elements")
+    for at in (0, 5, 6):
+        args = [16] * 7
+        args[at] = 18
+        refused(lib.thor_b200_checkpointed_activation_backward_launch(C.byref(a), *args, None), "not aligned to its elements")
+    n = norm_desc(dtype=int(DataType.fp32), param_dtype=int(DataType.fp32), grad_param_dtype=int(DataType.fp32))
+    for at in range(8):
+        args = [16] * 8
+        args[at] = 18
+        refused(lib.thor_b200_layernorm_launch(C.byref(n), *args, None, None, None), "not aligned to its elements")
+    for at in (0, 1, 2, 3, 6, 7, 8, 9, 10):
+        args = [16, 16, 16, 16, None, None, 16, 16, 16, 16, 16]
+        args[at] = 18
+        refused(lib.thor_b200_layernorm_backward_launch(C.byref(n), *args, 16, 1 << 30, None), "not aligned to its elements")
+
+
+def test_launch_counts():
+    count = lib.thor_b200_layernorm_backward_launch_count
+    assert [count(C.byref(norm_desc(cols=c)), p) for c, p in ((64, 0), (64, 1), (8192, 1), (8193, 1), (8193, 0))] == [1, 2, 2, 3, 1]
+    assert count(C.byref(norm_desc(rows=0)), 1) == 0 and count(None, 1) == 0

@@ -209,3 +209,29 @@ def test_refusals():
     shared = torch.zeros(8 * 16, device="cuda")
     refused(lambda: CheckpointPack().stamp(shared.reshape(8, 16), ActivationCheckpoint(shared.view(torch.float8_e4m3fn)[:128].reshape(8, 16), ck.scales[:, :1].contiguous(), 16)),
             "overlaps")
+
+
+def test_more_rows_than_a_grid_dimension_holds():
+    """Rows of 2048 columns and more have CTAs of their own up to 65535 rows; beyond that they share them."""
+    rows, cols = 65536 + 3, 2050
+    x = torch.randn(rows, cols, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).bfloat16()
+    ck = CheckpointPack().stamp(x).run()
+    for part in (slice(0, 5), slice(65530, rows)):
+        codes, scales = pack64(x[part].double(), torch.float8_e4m3fn)
+        assert torch.equal(ck.codes[part].double(), codes) and torch.equal(ck.scales[part].view(torch.uint8), scales)
+    back = CheckpointUnpack().stamp(ck).run()
+    assert torch.equal(back[-9:], unpack64(ck.codes[-9:], ck.scales[-9:], cols).bfloat16())
+
+
+def test_more_chunks_than_32_bits_count():
+    """2^31 + 5 rows of one column: two chunks a row, so their number passes 2^32."""
+    rows = (1 << 31) + 5
+    free, _ = torch.cuda.mem_get_info()
+    if free < 60 << 30:
+        pytest.skip("needs 60 GB")
+    x = torch.zeros(rows, 1, dtype=torch.float16, device="cuda")
+    x[-4:, 0] = torch.tensor([1.5, -3.0, 0.0, 100.0], dtype=torch.float16, device="cuda")
+    ck = CheckpointPack().stamp(x).run()
+    codes, scales = pack64(x[-4:].double(), torch.float8_e4m3fn)
+    assert torch.equal(ck.codes[-4:].double(), codes) and torch.equal(ck.scales[-4:].view(torch.uint8), scales)
+    assert not ck.codes[-(1 << 20):-4].view(torch.uint8).any() and not ck.scales[-(1 << 20):-4].view(torch.uint8).any()

@@ -288,6 +288,8 @@ int thor_b200_layernorm_launch(const thor_b200_layernorm_desc* d, const void* x,
         if (int st = checkPointer(who, p, dtypeSize(d->dtype))) return st;
     for (const void* p : {gamma, beta})
         if (int st = checkPointer(who, p, dtypeSize(d->param_dtype))) return st;
+    for (const void* p : {static_cast<const void*>(mean), static_cast<const void*>(rstd)})
+        if (int st = checkPointer(who, p, sizeof(float))) return st;
     if (int st = checkKept(who, codes, scales, *d)) return st;
     const bool aligned = d->cols % kVec == 0 && rowsAligned(x, d->x_stride, d->dtype, d->rows) && rowsAligned(residual, d->residual_stride, d->dtype, d->rows) &&
                          rowsAligned(y, d->y_stride, d->dtype, d->rows) && rowsAligned(sum, d->cols, d->dtype, d->rows);

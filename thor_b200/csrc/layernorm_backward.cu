@@ -397,6 +397,10 @@ int thor_b200_layernorm_backward_launch(const thor_b200_layernorm_desc* d, const
     for (const void* q : {grad_output, x, grad_sum, static_cast<const void*>(grad_input)})
         if (int st = checkPointer(who, q, dtypeSize(d->dtype))) return st;
     if (int st = checkPointer(who, gamma, dtypeSize(d->param_dtype))) return st;
+    for (const void* q : {static_cast<const void*>(mean), static_cast<const void*>(rstd)})
+        if (int st = checkPointer(who, q, sizeof(float))) return st;
+    for (const void* q : {static_cast<const void*>(grad_gamma), static_cast<const void*>(grad_beta)})
+        if (int st = checkPointer(who, q, dtypeSize(d->grad_param_dtype))) return st;
     if (int st = checkKept(who, codes, scales, *d)) return st;
     TB_REQUIRE((codes != nullptr) != (x != nullptr) && (x != nullptr) == (mean != nullptr), "%s: needs either the saved input with its mean or the checkpoint", who);
     const Plan p = planOf(d->rows, d->cols);
