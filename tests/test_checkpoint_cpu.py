@@ -111,7 +111,8 @@ def test_backward_workspace_holds_two_partial_rows_per_slab_and_stays_small(rows
     size = C.c_size_t()
     native.check(lib.thor_b200_layernorm_backward_workspace_bytes(C.byref(norm_desc(rows=rows, cols=cols)), C.byref(size)))
     one = 2 * ((cols + 7) // 8 * 8) * 4
-    assert size.value >= 16 and (size.value >= one) and size.value <= max(one, 64 << 20)
+    few = rows <= 512 and cols <= 8192  # one launch, no partial rows
+    assert size.value == 16 if few else one <= size.value <= max(one, 64 << 20)
 
 
 def test_python_refusals_without_a_gpu():
@@ -155,5 +156,6 @@ def test_pointers_off_their_elements():
 
 def test_launch_counts():
     count = lib.thor_b200_layernorm_backward_launch_count
-    assert [count(C.byref(norm_desc(cols=c)), p) for c, p in ((64, 0), (64, 1), (8192, 1), (8193, 1), (8193, 0))] == [1, 2, 2, 3, 1]
+    assert [count(C.byref(norm_desc(rows=r, cols=c)), p) for r, c, p in ((4, 64, 0), (4, 64, 1), (513, 64, 0), (513, 64, 1), (512, 8192, 1), (513, 8192, 1), (4, 8193, 1),
+                                                                         (4, 8193, 0))] == [1, 1, 1, 2, 1, 2, 3, 1]
     assert count(C.byref(norm_desc(rows=0)), 1) == 0 and count(None, 1) == 0

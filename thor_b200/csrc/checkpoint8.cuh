@@ -311,17 +311,40 @@ __device__ __forceinline__ void cutRow(uint32_t col, uint32_t cols, float2 (&v)[
     }
 }
 
-// The sixteen values that fetch16 of the same arguments has loaded; zero past the row's end.
-template <class T, bool ALIGNED>
+// The words from element m on, by selection: for warps whose lanes hold many rows, each with an m of its own.
+template <class T>
+__device__ __forceinline__ void selectWords(const uint32_t (&raw)[kRegs<T> / 2 * 3], uint32_t m, uint32_t (&w)[kRegs<T>]) {
+    constexpr int W = kRegs<T> / 2, N = kRegs<T>;
+    uint32_t r[W * 3];
+#pragma unroll
+    for (int i = 0; i < W * 3; ++i) r[i] = raw[i];
+#pragma unroll
+    for (int s = W / 2; s >= 1; s /= 2) {  // shift by s registers where m asks for it; what a later shift needs is kept
+#pragma unroll
+        for (int i = 0; i + s < W * 3; ++i) r[i] = (m * sizeof(T) / 4) & s ? r[i + s] : r[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = r[i];
+        else w[i] = __funnelshift_r(r[i], r[i + 1], (m % 2) * 16);
+    }
+}
+
+// The sixteen values that fetch16 of the same arguments has loaded; zero past the row's end.  MIXED: the lanes of a warp hold many rows.
+template <class T, bool ALIGNED, bool MIXED = false>
 __device__ __forceinline__ void expand16(const T* p, uint32_t col, uint32_t cols, const Raw<T, ALIGNED>& raw, float2 (&v)[8]) {
     if constexpr (ALIGNED) {
         widen16<T>(raw.w, v);
     } else {
         uint32_t w[kRegs<T>];
-        byOffset<T>(p, [&](auto m) {
+        if constexpr (MIXED) {
+            selectWords<T>(raw.w, (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) / sizeof(T)) % 8, w);
+        } else {
+            byOffset<T>(p, [&](auto m) {
 #pragma unroll
-            for (int i = 0; i < kRegs<T>; ++i) w[i] = wordAt<T>(raw.w, decltype(m)::value + i * static_cast<int>(4 / sizeof(T)));
-        });
+                for (int i = 0; i < kRegs<T>; ++i) w[i] = wordAt<T>(raw.w, decltype(m)::value + i * static_cast<int>(4 / sizeof(T)));
+            });
+        }
         widen16<T>(w, v);
         cutRow(col, cols, v);
     }

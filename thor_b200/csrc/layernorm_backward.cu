@@ -2,8 +2,8 @@
 //
 // Rows of up to 8192 columns: one persistent CTA an SM, whose teams walk their rows.  A thread owns sixteen columns for the whole kernel and
 // keeps their two column sums in registers; per row it needs one exchange with its team, for the two row sums.  At the end the CTA adds its
-// teams and leaves one partial row of each sum in the workspace, and a second kernel adds the partial rows in order.  Longer rows take two
-// kernels that read the row twice and once more.
+// teams and leaves one partial row of each sum in the workspace, and a second kernel adds the partial rows in order.  Up to 512 rows take one
+// launch whose CTAs share the two tasks.  Rows of more columns take two kernels that read the row twice and once more.
 #include <algorithm>
 
 #include "layernorm_common.cuh"
@@ -39,8 +39,9 @@ template <bool KEPT, bool ALIGNED, class T>
 struct Normal {
     Raw<T, ALIGNED> raw;
     __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetch16(b.x, b.x.p + row * b.x.stride + col, col, cols, raw); }
+    template <bool MIXED = false>
     __device__ __forceinline__ void expand(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols, float mean, float rstd, float2 (&n)[8]) const {
-        expand16(b.x.p + row * b.x.stride + col, col, cols, raw, n);
+        expand16<T, ALIGNED, MIXED>(b.x.p + row * b.x.stride + col, col, cols, raw, n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) n[i] = mul2(add2(n[i], both(-mean)), both(rstd));
     }
@@ -49,6 +50,7 @@ template <bool ALIGNED, class T>
 struct Normal<true, ALIGNED, T> {
     RawCodes raw;
     __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetchCodes(codesAt(b.kept, row, col), scaleAt(b.kept, row, col), col, cols, raw); }
+    template <bool MIXED = false>
     __device__ __forceinline__ void expand(const Backward<T>& b, uint64_t, uint32_t col, uint32_t cols, float, float, float2 (&n)[8]) const {
         expandCodes<!ALIGNED>(b.kept.code, col, cols, raw, n);
     }
@@ -180,6 +182,104 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
     }
 }
 
+// Few rows: one launch in which some CTAs take rows, as above but without column sums, and the others take the sums of 64 columns over all rows and
+// round them.  The rows are read twice, from L2, but no partial rows are written and no second kernel waits for them.
+constexpr uint32_t kStripLanes = 4, kStrip = kStripLanes * kVec;  // columns of a CTA; the other lanes of a warp take other rows
+
+template <class T, bool KEPT, bool ALIGNED, class O>
+__device__ __forceinline__ void columnStrip(const Backward<T>& b, uint32_t strip, float (&part)[kMaxThreads / 32][2][kStrip], O* grad_gamma, O* grad_beta) {
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+    const uint32_t col = strip * kStrip + lane % kStripLanes * kVec, step = warps * (32 / kStripLanes);
+    constexpr int kRows = ALIGNED || sizeof(T) == 2 ? 2 : 1;  // loaded before the first is used
+    float2 dg[8], db[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dg[i] = db[i] = both(0.0f);
+    for (uint32_t first = warp * (32 / kStripLanes) + lane / kStripLanes; first < b.rows; first += kRows * step) {
+        Raw<T, ALIGNED> grad[kRows];
+        Normal<KEPT, ALIGNED, T> normal[kRows];
+        float mean[kRows], rstd[kRows];
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const uint32_t row = first + k * step;
+            const bool there = row < b.rows;
+            fetch16(b.grad, b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col, col, there ? b.cols : 0, grad[k]);
+            normal[k].fetch(b, row, col, there ? b.cols : 0);
+            mean[k] = KEPT || !there ? 0.0f : b.mean[row];
+            rstd[k] = KEPT || !there ? 0.0f : b.rstd[row];
+        }
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const uint32_t row = first + k * step, cols = row < b.rows ? b.cols : 0;
+            float2 d[8], n[8];
+            expand16<T, ALIGNED, true>(b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col, col, cols, grad[k], d);
+            normal[k].template expand<true>(b, row, col, cols, mean[k], rstd[k], n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                dg[i] = fma2(d[i], n[i], dg[i]);
+                db[i] = add2(db[i], d[i]);
+            }
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float2 v = which == 0 ? dg[i] : db[i];
+#pragma unroll
+            for (int o = kStripLanes; o < 32; o *= 2) v = add2(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+            if (lane < kStripLanes) *reinterpret_cast<float2*>(&part[warp][which][lane * kVec + 2 * i]) = v;
+        }
+    }
+    __syncthreads();
+    for (uint32_t j = threadIdx.x; j < 2 * kStrip; j += blockDim.x) {
+        const uint32_t which = j / kStrip, c = strip * kStrip + j % kStrip;
+        if (c >= b.cols) continue;
+        float s = 0.0f;
+        for (uint32_t k = 0; k < warps; ++k) s += part[k][which][j % kStrip];
+        (which == 0 ? grad_gamma : grad_beta)[c] = static_cast<O>(s);
+    }
+}
+
+template <class T, bool KEPT, bool ALIGNED>
+__global__ void __launch_bounds__(kMaxThreads, 1) backwardFewRowsKernel(const __grid_constant__ Backward<T> b, uint32_t row_ctas, int grad_param_dtype, void* grad_gamma, void* grad_beta) {
+    __shared__ union {
+        Scratch scratch;
+        float part[kMaxThreads / 32][2][kStrip];
+    } shared;
+    gridDependencyWait();
+    gridLaunchDependents();
+    if (blockIdx.x >= row_ctas) {
+        const uint32_t strip = blockIdx.x - row_ctas;
+        if (grad_param_dtype == THOR_B200_FP32) columnStrip<T, KEPT, ALIGNED>(b, strip, shared.part, static_cast<float*>(grad_gamma), static_cast<float*>(grad_beta));
+        else if (grad_param_dtype == THOR_B200_FP16) columnStrip<T, KEPT, ALIGNED>(b, strip, shared.part, static_cast<__half*>(grad_gamma), static_cast<__half*>(grad_beta));
+        else columnStrip<T, KEPT, ALIGNED>(b, strip, shared.part, static_cast<__nv_bfloat16*>(grad_gamma), static_cast<__nv_bfloat16*>(grad_beta));
+        return;
+    }
+    const uint32_t team = b.team, team_id = threadIdx.x / team, t = threadIdx.x - team_id * team, teams = blockDim.x / team;
+    const uint32_t lane = threadIdx.x % 32, col = t * kVec;
+    const bool before = team < 32 ? t > 0 : lane > 0, after = team < 32 ? t + 1 < team : lane < 31;
+    const uint32_t step = row_ctas * teams;
+    int slot = 0;
+    for (uint32_t base = blockIdx.x * teams; base < b.rows; base += step) {
+        const uint32_t row = base + team_id, cols = row < b.rows ? b.cols : 0;
+        Raw<T, ALIGNED> grad, stream;
+        Normal<KEPT, ALIGNED, T> normal;
+        const T* const grad_at = b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col;
+        fetch16(b.grad, grad_at, col, cols, grad);
+        normal.fetch(b, row, col, cols);
+        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + static_cast<uint64_t>(row) * b.grad_sum.stride + col, col, cols, stream);
+        const float rstd = cols > 0 ? b.rstd[row] : 0.0f, mean = cols > 0 && !KEPT ? b.mean[row] : 0.0f;
+        float2 w[8], n[8], s1 = both(0.0f), s2 = both(0.0f);
+        expand16(grad_at, col, cols, grad, w);
+        normal.expand(b, row, col, cols, mean, rstd, n);
+        weigh16(b, col, cols, w, n, s1, s2);
+        const float2 s = teamSum(make_float2(s1.x + s1.y, s2.x + s2.y), team, team_id, shared.scratch, slot);
+        slot ^= 1;
+        finish16<ALIGNED>(b, row, col, cols, w, n, s.x * b.inverse, s.y * b.inverse, rstd, stream, before, after);
+    }
+}
+
 // ---- rows longer than 8192 columns ----------------------------------------------------------------------------
 // One CTA a row, two passes over it (the second mostly from L2).
 template <class T, bool KEPT, bool ALIGNED>
@@ -295,14 +395,19 @@ __global__ void __launch_bounds__(256) foldKernel(const float* __restrict__ part
 }
 
 // ---- host side --------------------------------------------------------------------------------------------
+// Up to here one launch is faster than two: [128, 4096] bf16 4.8 us against 10.6, [512, 4096] 7.8 against 13.0, [512, 8192] 10.9 against 12.0,
+// [1024, 8192] 20.4 against 15.1.
+constexpr uint64_t kFewRows = 512;
+
 struct Plan {
-    bool fused;
+    bool fused, few;
     uint32_t team, teams, partial_rows, padded;
     uint64_t slab_rows;
 };
 Plan planOf(uint64_t rows, uint64_t cols) {
     Plan p{};
     p.fused = cols <= kFusedCols;
+    p.few = p.fused && rows <= kFewRows;
     if (p.fused) {
         p.team = teamOf((cols + kVec - 1) / kVec, 1);
         p.teams = kMaxThreads / p.team;
@@ -330,6 +435,12 @@ int launchBackward(const Backward<T>& b, const Plan& p, bool aligned, int grad_p
     const int st = byFlag(aligned, [&](auto a) {
         return byFlag(b.kept.codes != nullptr, [&](auto k) {
             constexpr bool A = decltype(a)::value, K = decltype(k)::value;
+            if (p.few && b.partial != nullptr) {
+                TB_CUDA(launchDependent(backwardFewRowsKernel<T, K, A>, dim3(p.partial_rows + (b.cols + kStrip - 1) / kStrip), dim3(p.team * p.teams), 0, stream,
+                                        b, p.partial_rows, grad_param_dtype, grad_gamma, grad_beta));
+                countLaunch();
+                return static_cast<int>(THOR_B200_OK);
+            }
             if (p.fused) {
                 TB_CUDA(launchDependent(backwardKernel<T, K, A>, dim3(p.partial_rows), dim3(p.team * p.teams), 0, stream, b));
                 countLaunch();
@@ -343,7 +454,7 @@ int launchBackward(const Backward<T>& b, const Plan& p, bool aligned, int grad_p
             return static_cast<int>(THOR_B200_OK);
         });
     });
-    if (st || b.partial == nullptr) return st;
+    if (st || b.partial == nullptr || p.few) return st;
     switch (grad_param_dtype) {
         case THOR_B200_FP32: return launchFold<float>(b.partial, p, b.cols, grad_gamma, grad_beta, stream);
         case THOR_B200_FP16: return launchFold<__half>(b.partial, p, b.cols, grad_gamma, grad_beta, stream);
@@ -361,13 +472,14 @@ int thor_b200_layernorm_backward_workspace_bytes(const thor_b200_layernorm_desc*
     TB_REQUIRE(bytes != nullptr, "layernorm_backward_workspace_bytes: null argument");
     if (int st = ln::checkDesc("layernorm_backward_workspace_bytes", d)) return st;
     const Plan p = planOf(d->rows, d->cols);
-    *bytes = std::max<size_t>(16, static_cast<size_t>(p.partial_rows) * 2 * p.padded * sizeof(float));
+    *bytes = p.few ? 16 : std::max<size_t>(16, static_cast<size_t>(p.partial_rows) * 2 * p.padded * sizeof(float));
     return THOR_B200_OK;
 }
 
 int thor_b200_layernorm_backward_launch_count(const thor_b200_layernorm_desc* d, int parameter_gradients) {
     if (d == nullptr || d->rows == 0) return 0;
-    return !parameter_gradients ? 1 : (tb::planOf(d->rows, d->cols).fused ? 2 : 3);
+    const tb::Plan p = tb::planOf(d->rows, d->cols);
+    return !parameter_gradients || p.few ? 1 : (p.fused ? 2 : 3);
 }
 
 int thor_b200_layernorm_backward_launch(const thor_b200_layernorm_desc* d, const void* grad_output, const void* x, const float* mean, const float* rstd,
