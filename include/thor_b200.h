@@ -480,14 +480,14 @@ THOR_B200_API void thor_b200_rowprog_destroy(thor_b200_rowprog* prog);
  * to the nearest code, ties to even: the error is at most half a step of the code.  A block that holds an infinity or a
  * NaN gets scale 255 and codes zero and unpacks as NaN throughout, so an overflow stays visible in the backward pass.
  * Rows are independent: a range of rows of the two arrays is the checkpoint of that range.
- * Tensors are [rows, cols] with neighbouring columns adjacent and `stride` elements between rows (any stride >= cols; the
- * vectorised path needs 16-byte aligned rows and cols % 8 == 0).  rows == 0 is a no-op.  Outputs must not overlap inputs.
+ * Tensors are [rows, cols] with neighbouring columns adjacent and `stride` elements between rows (any stride in [cols, 2^32);
+ * rows that start on 32 bytes and have a multiple of 16 columns take the shortest path).  rows == 0 is a no-op.  Outputs must not overlap inputs.
  * No workspace, no allocation.  No counterpart in the reference, which keeps activations in full.
  * ------------------------------------------------------------------------------------------- */
 typedef struct thor_b200_checkpoint_desc {
     int32_t dtype;      /* fp32 / fp16 / bf16: the tensor */
     int32_t code_dtype; /* fp8_e4m3 / fp8_e5m2 / int8 */
-    uint64_t rows, cols; /* cols in [1, 2^31) */
+    uint64_t rows, cols; /* rows below 2^32, cols in [1, 2^31) */
     int64_t stride;     /* elements between the tensor's rows (ignored for one row) */
 } thor_b200_checkpoint_desc;
 
@@ -546,7 +546,7 @@ typedef struct thor_b200_layernorm_desc {
     int32_t code_dtype;       /* fp8_e4m3 / fp8_e5m2 / int8, 0: no checkpoint */
     float eps;                /* forward; >= 0 */
     uint32_t reserved;        /* must be zero */
-    uint64_t rows, cols;      /* cols in [1, 2^31) */
+    uint64_t rows, cols;      /* rows below 2^31, cols in [1, 2^31) */
     int64_t x_stride;         /* elements between rows of x and, in the backward pass, of the saved x */
     int64_t residual_stride;  /* of residual; backward: of grad_sum */
     int64_t y_stride;         /* of y; backward: of grad_output.  sum and grad_input are dense. */
@@ -559,7 +559,7 @@ THOR_B200_API int thor_b200_layernorm_backward_launch(const thor_b200_layernorm_
                                                       const float* rstd, const void* codes, const void* scales, const void* gamma, const void* grad_sum,
                                                       void* grad_input, void* grad_gamma, void* grad_beta, void* workspace, size_t workspace_bytes,
                                                       void* stream);
-/* Kernels one backward launch issues. */
+/* Kernels one backward launch issues (parameter_gradients: whether grad_gamma and grad_beta are asked for). */
 THOR_B200_API int thor_b200_layernorm_backward_launch_count(const thor_b200_layernorm_desc* desc, int parameter_gradients);
 
 /* ---------------------------------------------------------------------------------------------

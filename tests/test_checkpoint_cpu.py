@@ -27,7 +27,8 @@ def test_pitches():
 
 @pytest.mark.parametrize("change,text", [
     (dict(dtype=int(DataType.fp64)), "fp32, fp16 or bf16"), (dict(dtype=E4M3), "fp32, fp16 or bf16"), (dict(code_dtype=int(DataType.uint8)), "fp8_e4m3, fp8_e5m2 or int8"),
-    (dict(cols=0), "columns"), (dict(cols=1 << 31), "columns"), (dict(stride=63), "row stride"), (dict(stride=-64), "row stride"), (dict(rows=1 << 61), "overflows"),
+    (dict(cols=0), "columns"), (dict(cols=1 << 31), "columns"), (dict(stride=63), "row stride"), (dict(stride=-64), "row stride"), (dict(stride=1 << 32), "2\\^32"), (dict(rows=1 << 61), "overflows"),
+    (dict(rows=1 << 32), "2\\^32 - 1 rows"),
 ])
 def test_pack_and_unpack_descriptions(change, text):
     d = _CheckpointDesc(**{**dict(dtype=BF16, code_dtype=E4M3, rows=4, cols=64, stride=64), **change})
@@ -49,7 +50,7 @@ def test_pack_pointers():
 
 @pytest.mark.parametrize("change,text", [
     (dict(kind=2), "unknown activation"), (dict(dtype=int(DataType.int8)), "fp32, fp16 or bf16"), (dict(code_dtype=0), "fp8_e4m3"), (dict(x_stride=1), "stride of x"),
-    (dict(gate_stride=1), "stride of gate"), (dict(y_stride=1), "stride of y"), (dict(cols=0), "columns"),
+    (dict(gate_stride=1), "stride of gate"), (dict(y_stride=1), "stride of y"), (dict(cols=0), "columns"), (dict(gate_stride=1 << 33), "2\\^32"),
 ])
 def test_activation_descriptions(change, text):
     d = _ActivationDesc(**{**dict(kind=0, gated=1, dtype=BF16, code_dtype=E4M3, rows=4, cols=64, x_stride=128, gate_stride=128, y_stride=64), **change})
@@ -77,7 +78,7 @@ def norm_desc(**change):
 @pytest.mark.parametrize("change,text", [
     (dict(dtype=E4M3), "tensors must be"), (dict(param_dtype=int(DataType.fp64)), "parameters must be"), (dict(code_dtype=int(DataType.uint8)), "codes must be"),
     (dict(reserved=1), "reserved"), (dict(cols=0), "columns"), (dict(rows=1 << 31), "rows"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
-    (dict(x_stride=63), "stride of x"), (dict(y_stride=63), "row stride of"),
+    (dict(x_stride=63), "stride of x"), (dict(y_stride=63), "row stride of"), (dict(x_stride=1 << 32), "2\\^32"),
 ])
 def test_layernorm_descriptions(change, text):
     d = norm_desc(**change)

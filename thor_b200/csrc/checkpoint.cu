@@ -11,27 +11,25 @@ template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) packKernel(Rows<T> x, Writer out, Walk w) {
     gridDependencyWait();
     gridLaunchDependents();
-    uint64_t row;
-    uint32_t col, cols;
+    uint32_t row, col, cols;
     locate(w, row, col, cols);
     float2 v[8];
-    load16<ALIGNED>(x, x.p + row * x.stride + col, col, cols, v);
+    load16<ALIGNED>(x, x.p + rowStart(row, x.stride) + col, col, cols, v);
     writeCodes(codesAt(out, row, col), scaleAt(out, row, col), out.code, col, cols, v);
 }
 
 template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) unpackKernel(Reader in, T* __restrict__ y, int64_t y_stride, Walk w) {
+__global__ void __launch_bounds__(kThreads) unpackKernel(Reader in, T* __restrict__ y, uint32_t y_stride, Walk w) {
     gridDependencyWait();
     gridLaunchDependents();
-    uint64_t row;
-    uint32_t col, cols;
+    uint32_t row, col, cols;
     locate(w, row, col, cols);
     RawCodes raw;
     fetchCodes(codesAt(in, row, col), scaleAt(in, row, col), col, cols, raw);
     float2 v[8];
     expandCodes<false>(in.code, col, cols, raw, v);  // columns past the row's end are not stored
     const uint32_t lane = threadIdx.x % 32;
-    store16<ALIGNED>(y + row * y_stride + col, col, cols, v, lane > 0 && col > 0, lane < 31);
+    store16<ALIGNED>(y + rowStart(row, y_stride) + col, col, cols, v, lane > 0 && col > 0, lane < 31);
 }
 
 }  // namespace
@@ -48,7 +46,7 @@ int thor_b200_checkpoint_pack_launch(const thor_b200_checkpoint_desc* d, const v
     const char* who = "checkpoint_pack";
     TB_REQUIRE(d != nullptr, "%s: null description", who);
     if (int st = checkShape(who, d->dtype, d->code_dtype, d->rows, d->cols)) return st;
-    if (int st = checkStride(who, "the tensor", d->stride, d->rows, d->cols)) return st;
+    if (int st = checkRowStride(who, "the tensor", d->stride, d->rows, d->cols)) return st;
     if (d->rows == 0) return THOR_B200_OK;
     if (int st = checkTensor(who, x, d->dtype)) return st;
     if (int st = checkCheckpoint(who, codes, scales)) return st;
@@ -74,7 +72,7 @@ int thor_b200_checkpoint_unpack_launch(const thor_b200_checkpoint_desc* d, const
     const char* who = "checkpoint_unpack";
     TB_REQUIRE(d != nullptr, "%s: null description", who);
     if (int st = checkShape(who, d->dtype, d->code_dtype, d->rows, d->cols)) return st;
-    if (int st = checkStride(who, "the tensor", d->stride, d->rows, d->cols)) return st;
+    if (int st = checkRowStride(who, "the tensor", d->stride, d->rows, d->cols)) return st;
     if (d->rows == 0) return THOR_B200_OK;
     if (int st = checkTensor(who, y, d->dtype)) return st;
     if (int st = checkCheckpoint(who, codes, scales)) return st;
@@ -87,7 +85,7 @@ int thor_b200_checkpoint_unpack_launch(const thor_b200_checkpoint_desc* d, const
     return byDtype(d->dtype, [&](auto t) {
         using T = decltype(t);
         return byFlag(aligned, [&](auto a) {
-            TB_CUDA(launchDependent(unpackKernel<T, decltype(a)::value>, grid, block, 0, stream, in, static_cast<T*>(y), d->stride, w));
+            TB_CUDA(launchDependent(unpackKernel<T, decltype(a)::value>, grid, block, 0, stream, in, static_cast<T*>(y), strideOf(d->stride, d->rows), w));
             countLaunch();
             return static_cast<int>(THOR_B200_OK);
         });

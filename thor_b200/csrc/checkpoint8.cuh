@@ -199,11 +199,14 @@ __device__ __forceinline__ void narrow16(const float2 (&v)[8], uint32_t (&w)[kRe
     }
 }
 
+// Where a row starts: the product passes 32 bits, its factors do not.
+__device__ __forceinline__ uint64_t rowStart(uint32_t row, uint32_t stride) { return static_cast<uint64_t>(row) * stride; }
+
 // Rows of a tensor that is read.
 template <class T>
 struct Rows {
     const T* p;
-    int64_t stride;   // elements between rows
+    uint32_t stride;  // elements between rows
     const void* end;  // one past the last element
 };
 
@@ -445,18 +448,18 @@ __device__ __forceinline__ void roundTo16(float2 (&v)[8]) {
 struct Writer {
     uint8_t* codes;
     uint8_t* scales;
-    uint64_t code_pitch, scale_pitch;
+    uint32_t code_pitch, scale_pitch;
     int code;
 };
 struct Reader {
     const uint8_t* codes;
     const uint8_t* scales;
-    uint64_t code_pitch, scale_pitch;
+    uint32_t code_pitch, scale_pitch;
     int code;
 };
 
-__device__ __forceinline__ uint8_t* codesAt(const Writer& w, uint64_t row, uint32_t col) { return w.codes + row * w.code_pitch + col; }
-__device__ __forceinline__ uint8_t* scaleAt(const Writer& w, uint64_t row, uint32_t col) { return w.scales + row * w.scale_pitch + col / kBlock; }
+__device__ __forceinline__ uint8_t* codesAt(const Writer& w, uint32_t row, uint32_t col) { return w.codes + rowStart(row, w.code_pitch) + col; }
+__device__ __forceinline__ uint8_t* scaleAt(const Writer& w, uint32_t row, uint32_t col) { return w.scales + rowStart(row, w.scale_pitch) + col / kBlock; }
 
 // Sixteen columns of one row by every lane, zero past the row's end; lanes 2 k and 2 k + 1 hold one block.  All 32 lanes call it, with cols = 0
 // where a lane has no row.
@@ -470,8 +473,8 @@ struct RawCodes {
     uint4 codes;
     uint32_t scale;
 };
-__device__ __forceinline__ const uint8_t* codesAt(const Reader& r, uint64_t row, uint32_t col) { return r.codes + row * r.code_pitch + col; }
-__device__ __forceinline__ const uint8_t* scaleAt(const Reader& r, uint64_t row, uint32_t col) { return r.scales + row * r.scale_pitch + col / kBlock; }
+__device__ __forceinline__ const uint8_t* codesAt(const Reader& r, uint32_t row, uint32_t col) { return r.codes + rowStart(row, r.code_pitch) + col; }
+__device__ __forceinline__ const uint8_t* scaleAt(const Reader& r, uint32_t row, uint32_t col) { return r.scales + rowStart(row, r.scale_pitch) + col / kBlock; }
 __device__ __forceinline__ void fetchCodes(const uint8_t* codes, const uint8_t* scale, uint32_t col, uint32_t cols, RawCodes& raw) {
     raw.codes = make_uint4(0u, 0u, 0u, 0u);
     raw.scale = 0;
@@ -491,10 +494,17 @@ __device__ __forceinline__ void expandCodes(int code, uint32_t col, uint32_t col
 inline bool rowsAligned(const void* p, int64_t stride, int dtype, uint64_t rows) {
     return p == nullptr || (isAligned(p, 32) && (rows <= 1 || (static_cast<uint64_t>(stride) * dtypeSize(dtype)) % 32 == 0));
 }
+// The stride of checked arguments; one row has none.
+inline uint32_t strideOf(int64_t stride, uint64_t rows) { return rows > 1 ? static_cast<uint32_t>(stride) : 0u; }
+inline int checkRowStride(const char* who, const char* what, int64_t stride, uint64_t rows, uint64_t cols) {
+    TB_REQUIRE(rows <= 1 || (stride >= 0 && static_cast<uint64_t>(stride) >= cols), "%s: the row stride of %s is smaller than a row", who, what);
+    TB_REQUIRE(rows <= 1 || stride <= 0xffffffffll, "%s: the row stride of %s is 2^32 elements or more", who, what);
+    return THOR_B200_OK;
+}
 template <class T>
 Rows<T> rowsOf(const void* p, int64_t stride, uint64_t rows, uint64_t cols) {
     const T* t = static_cast<const T*>(p);
-    return Rows<T>{t, stride, t == nullptr ? nullptr : t + (rows - 1) * static_cast<uint64_t>(rows > 1 ? stride : 0) + cols};
+    return Rows<T>{t, strideOf(stride, rows), t == nullptr ? nullptr : t + (rows - 1) * static_cast<uint64_t>(strideOf(stride, rows)) + cols};
 }
 template <class F>
 int byDtype(int dtype, F&& f) {

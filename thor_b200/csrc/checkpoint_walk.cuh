@@ -20,7 +20,7 @@ struct Walk {
     bool row_a_cta;
 };
 // This thread's chunk; cols = 0 where there is none left.
-__device__ __forceinline__ void locate(const Walk& w, uint64_t& row, uint32_t& col, uint32_t& cols) {
+__device__ __forceinline__ void locate(const Walk& w, uint32_t& row, uint32_t& col, uint32_t& cols) {
     if (w.row_a_cta) {
         row = blockIdx.y;
         col = (blockIdx.x * blockDim.x + threadIdx.x) * kVec;
@@ -37,8 +37,8 @@ __device__ __forceinline__ void locate(const Walk& w, uint64_t& row, uint32_t& c
         row = r;
         col = (static_cast<uint32_t>(unit) - r * w.chunks) * kVec;
     } else {
-        row = unit / w.chunks;
-        col = static_cast<uint32_t>(unit - row * w.chunks) * kVec;
+        row = static_cast<uint32_t>(unit / w.chunks);
+        col = static_cast<uint32_t>(unit - static_cast<uint64_t>(row) * w.chunks) * kVec;
     }
 }
 
@@ -69,10 +69,7 @@ inline int checkShape(const char* who, int dtype, int code_dtype, uint64_t rows,
     TB_REQUIRE(codeDtypeOk(code_dtype), "%s: codes must be fp8_e4m3, fp8_e5m2 or int8, got %s", who, dtypeName(code_dtype));
     TB_REQUIRE(cols > 0 && cols <= 0x7fffffffull, "%s: rows must have 1 to 2^31 - 1 columns", who);
     TB_REQUIRE(rows <= (1ull << 62) / (cols + kBlock), "%s: rows * cols overflows", who);
-    return THOR_B200_OK;
-}
-inline int checkStride(const char* who, const char* what, int64_t stride, uint64_t rows, uint64_t cols) {
-    TB_REQUIRE(rows <= 1 || (stride >= 0 && static_cast<uint64_t>(stride) >= cols), "%s: the row stride of %s is smaller than a row", who, what);
+    TB_REQUIRE(rows <= 0xffffffffull, "%s: more than 2^32 - 1 rows", who);
     return THOR_B200_OK;
 }
 inline int checkTensor(const char* who, const void* p, int dtype) {
@@ -86,10 +83,10 @@ inline int checkCheckpoint(const char* who, const void* codes, const void* scale
     return THOR_B200_OK;
 }
 inline Writer writerOf(void* codes, void* scales, uint64_t cols, int code) {
-    return Writer{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), codePitch(cols), scalePitch(cols), code};
+    return Writer{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), static_cast<uint32_t>(codePitch(cols)), static_cast<uint32_t>(scalePitch(cols)), code};
 }
 inline Reader readerOf(const void* codes, const void* scales, uint64_t cols, int code) {
-    return Reader{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), codePitch(cols), scalePitch(cols), code};
+    return Reader{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<uint32_t>(codePitch(cols)), static_cast<uint32_t>(scalePitch(cols)), code};
 }
 inline bool denseRows(int64_t stride, uint64_t rows, uint64_t cols) { return rows <= 1 || static_cast<uint64_t>(stride) == cols; }
 

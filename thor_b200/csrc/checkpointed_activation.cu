@@ -64,15 +64,14 @@ __device__ __forceinline__ void activation2(float2 x, float2& value, float2& slo
 }
 
 template <class T, int KIND, bool GATED, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) activationKernel(Rows<T> x, Rows<T> gate, T* __restrict__ y, int64_t y_stride, Writer out, Writer gate_out, Walk w) {
+__global__ void __launch_bounds__(kThreads) activationKernel(Rows<T> x, Rows<T> gate, T* __restrict__ y, uint32_t y_stride, Writer out, Writer gate_out, Walk w) {
     gridDependencyWait();
     gridLaunchDependents();
-    uint64_t row;
-    uint32_t col, cols;
+    uint32_t row, col, cols;
     locate(w, row, col, cols);
     Raw<T, ALIGNED> raw, raw_gate;
-    const T* const x_at = x.p + row * x.stride + col;
-    const T* const gate_at = gate.p + row * gate.stride + col;
+    const T* const x_at = x.p + rowStart(row, x.stride) + col;
+    const T* const gate_at = gate.p + rowStart(row, gate.stride) + col;
     fetch16(x, x_at, col, cols, raw);
     if constexpr (GATED) fetch16(gate, gate_at, col, cols, raw_gate);
     float2 v[8], r[8];
@@ -90,20 +89,19 @@ __global__ void __launch_bounds__(kThreads) activationKernel(Rows<T> x, Rows<T> 
         for (int i = 0; i < 8; ++i) r[i] = mul2(r[i], v[i]);
     }
     const uint32_t lane = threadIdx.x % 32;
-    store16<ALIGNED>(y + row * y_stride + col, col, cols, r, lane > 0 && col > 0, lane < 31);
+    store16<ALIGNED>(y + rowStart(row, y_stride) + col, col, cols, r, lane > 0 && col > 0, lane < 31);
 }
 
 template <class T, int KIND, bool GATED, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) activationBackwardKernel(Rows<T> grad, Reader in, Reader gate_in, T* __restrict__ grad_x, int64_t grad_x_stride,
-                                                                     T* __restrict__ grad_gate, int64_t grad_gate_stride, Walk w) {
+__global__ void __launch_bounds__(kThreads) activationBackwardKernel(Rows<T> grad, Reader in, Reader gate_in, T* __restrict__ grad_x, uint32_t grad_x_stride,
+                                                                     T* __restrict__ grad_gate, uint32_t grad_gate_stride, Walk w) {
     gridDependencyWait();
     gridLaunchDependents();
-    uint64_t row;
-    uint32_t col, cols;
+    uint32_t row, col, cols;
     locate(w, row, col, cols);
     Raw<T, ALIGNED> raw;
     RawCodes codes, gate_codes;
-    const T* const grad_at = grad.p + row * grad.stride + col;
+    const T* const grad_at = grad.p + rowStart(row, grad.stride) + col;
     fetch16(grad, grad_at, col, cols, raw);
     fetchCodes(codesAt(in, row, col), scaleAt(in, row, col), col, cols, codes);
     if constexpr (GATED) fetchCodes(codesAt(gate_in, row, col), scaleAt(gate_in, row, col), col, cols, gate_codes);
@@ -120,22 +118,22 @@ __global__ void __launch_bounds__(kThreads) activationBackwardKernel(Rows<T> gra
     const uint32_t lane = threadIdx.x % 32;
     const bool before = lane > 0 && col > 0, after = lane < 31;
     if constexpr (GATED) {
-        store16<ALIGNED>(grad_gate + row * grad_gate_stride + col, col, cols, d, before, after);
+        store16<ALIGNED>(grad_gate + rowStart(row, grad_gate_stride) + col, col, cols, d, before, after);
         expandCodes<false>(gate_in.code, col, cols, gate_codes, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dx[i] = mul2(dx[i], v[i]);
     }
-    store16<ALIGNED>(grad_x + row * grad_x_stride + col, col, cols, dx, before, after);
+    store16<ALIGNED>(grad_x + rowStart(row, grad_x_stride) + col, col, cols, dx, before, after);
 }
 
 int checkActivation(const char* who, const thor_b200_checkpointed_activation_desc* d) {
     TB_REQUIRE(d != nullptr, "%s: null description", who);
     TB_REQUIRE(d->kind == THOR_B200_ACTIVATION_GELU || d->kind == THOR_B200_ACTIVATION_SWISH, "%s: unknown activation %d", who, d->kind);
     if (int st = checkShape(who, d->dtype, d->code_dtype, d->rows, d->cols)) return st;
-    if (int st = checkStride(who, "x", d->x_stride, d->rows, d->cols)) return st;
+    if (int st = checkRowStride(who, "x", d->x_stride, d->rows, d->cols)) return st;
     if (d->gated)
-        if (int st = checkStride(who, "gate", d->gate_stride, d->rows, d->cols)) return st;
-    return checkStride(who, "y", d->y_stride, d->rows, d->cols);
+        if (int st = checkRowStride(who, "gate", d->gate_stride, d->rows, d->cols)) return st;
+    return checkRowStride(who, "y", d->y_stride, d->rows, d->cols);
 }
 // The tensors that play x, gate and y (their gradients in the backward pass) and the checkpoints.
 int checkOperands(const char* who, const thor_b200_checkpointed_activation_desc& d, const void* x, const void* gate, const void* y, const void* codes, const void* scales,
@@ -189,7 +187,7 @@ int thor_b200_checkpointed_activation_launch(const thor_b200_checkpointed_activa
         using T = decltype(t);
         TB_CUDA(launchDependent(activationKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, block, 0,
                                 static_cast<cudaStream_t>(stream_v), rowsOf<T>(x, d->x_stride, d->rows, d->cols), rowsOf<T>(gate, d->gate_stride, d->rows, d->cols),
-                                static_cast<T*>(y), d->y_stride, out, gate_out, w));
+                                static_cast<T*>(y), strideOf(d->y_stride, d->rows), out, gate_out, w));
         countLaunch();
         return static_cast<int>(THOR_B200_OK);
     });
@@ -212,7 +210,7 @@ int thor_b200_checkpointed_activation_backward_launch(const thor_b200_checkpoint
         using T = decltype(t);
         TB_CUDA(launchDependent(activationBackwardKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, block, 0,
                                 static_cast<cudaStream_t>(stream_v), rowsOf<T>(grad_output, d->y_stride, d->rows, d->cols), in, gate_in, static_cast<T*>(grad_input),
-                                d->x_stride, static_cast<T*>(grad_gate), d->gate_stride, w));
+                                strideOf(d->x_stride, d->rows), static_cast<T*>(grad_gate), strideOf(d->gate_stride, d->rows), w));
         countLaunch();
         return static_cast<int>(THOR_B200_OK);
     });

@@ -26,12 +26,11 @@ struct Forward {
     T* sum;
     float* mean;
     float* rstd;
-    int64_t y_stride;
+    uint32_t y_stride;
     Param gamma, beta;
     bool packable;  // the parameters that are given have the tensors' type
     Writer kept;  // kept.codes == nullptr: no checkpoint
-    uint64_t rows;
-    uint32_t cols, team;
+    uint32_t rows, cols, team;
     float eps, count, inverse;  // count = cols, inverse = 1 / cols
 };
 
@@ -82,7 +81,7 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
     uint32_t row = blockIdx.x * teams + team_id;
     uint32_t cols = row < f.rows ? f.cols : 0;
     Raw<T, ALIGNED> next[CHUNKS], next_residual[RESIDUAL ? CHUNKS : 1];
-    auto at = [&](const Rows<T>& in, uint32_t r, int k) { return in.p + static_cast<uint64_t>(r) * in.stride + (t + k * team) * kVec; };
+    auto at = [&](const Rows<T>& in, uint32_t r, int k) { return in.p + rowStart(r, in.stride) + (t + k * team) * kVec; };
     auto fetch = [&](uint32_t r, uint32_t n) {
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
@@ -116,7 +115,7 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
         if constexpr (kAhead) fetch(row + step, next_cols);
         if constexpr (RESIDUAL) {
             if (f.sum != nullptr) {
-                T* const sum_at = f.sum + static_cast<uint64_t>(row) * f.cols + t * kVec;
+                T* const sum_at = f.sum + rowStart(row, f.cols) + t * kVec;
 #pragma unroll
                 for (int k = 0; k < CHUNKS; ++k) store16<ALIGNED>(sum_at + k * team * kVec, (t + k * team) * kVec, cols, v[k], before, after);
             }
@@ -147,7 +146,7 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
         for (int k = 0; k < CHUNKS; ++k) {
             const uint32_t col = (t + k * team) * kVec;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[k][i] = mul2(add2(v[k][i], both(shift)), both(rstd));
+            for (int i = 0; i < 8; ++i) v[k][i] = fma2(v[k][i], both(rstd), both(shift * rstd));
             if constexpr (!ALIGNED) cutRow(col, cols, v[k]);
             if (f.kept.codes != nullptr) writeCodes(codesAt(f.kept, row, col), scaleAt(f.kept, row, col), f.kept.code, col, cols, v[k]);
 #pragma unroll
@@ -158,7 +157,7 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[k][4 * h + i] = fma2(v[k][4 * h + i], g[i], b[i]);
             }
-            store16<ALIGNED>(f.y + static_cast<uint64_t>(row) * f.y_stride + col, col, cols, v[k], before, after);
+            store16<ALIGNED>(f.y + rowStart(row, f.y_stride) + col, col, cols, v[k], before, after);
         }
         cols = next_cols;
         if constexpr (!kAhead) fetch(row + step, cols);
@@ -167,11 +166,11 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
 
 // The row that is normalised: x, or the rounded sum.
 template <bool ALIGNED, class T>
-__device__ __forceinline__ void input16(const Forward<T>& f, uint64_t row, uint32_t col, uint32_t cols, float2 (&v)[8]) {
-    load16<ALIGNED>(f.x, f.x.p + row * f.x.stride + col, col, cols, v);
+__device__ __forceinline__ void input16(const Forward<T>& f, uint32_t row, uint32_t col, uint32_t cols, float2 (&v)[8]) {
+    load16<ALIGNED>(f.x, f.x.p + rowStart(row, f.x.stride) + col, col, cols, v);
     if (f.residual.p != nullptr) {
         float2 r[8];
-        load16<ALIGNED>(f.residual, f.residual.p + row * f.residual.stride + col, col, cols, r);
+        load16<ALIGNED>(f.residual, f.residual.p + rowStart(row, f.residual.stride) + col, col, cols, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = add2(v[i], r[i]);
         roundTo16<T>(v);
@@ -183,7 +182,7 @@ __global__ void __launch_bounds__(512) forwardLoopKernel(const __grid_constant__
     __shared__ float scratch[2][32];
     gridDependencyWait();
     gridLaunchDependents();
-    const uint64_t row = blockIdx.x;
+    const uint32_t row = blockIdx.x;
     const uint32_t lane = threadIdx.x % 32, step = blockDim.x * kVec;
     // the loops' trip counts are the same for the whole CTA; a thread past the row's end has columns of none
     float2 v[8];
@@ -193,7 +192,7 @@ __global__ void __launch_bounds__(512) forwardLoopKernel(const __grid_constant__
         const uint32_t col = static_cast<uint32_t>(at), cols = at < f.cols ? f.cols : 0;
         input16<ALIGNED>(f, row, col, cols, v);
         s += sum16(v);
-        if (f.sum != nullptr) store16<ALIGNED>(f.sum + row * f.cols + col, col, cols, v, lane > 0, lane < 31);
+        if (f.sum != nullptr) store16<ALIGNED>(f.sum + rowStart(row, f.cols) + col, col, cols, v, lane > 0, lane < 31);
     }
     const float mean = divideBy(ctaSum(s, scratch[0]), f.count, f.inverse);
     s = 0.0f;
@@ -222,7 +221,7 @@ __global__ void __launch_bounds__(512) forwardLoopKernel(const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * h + i] = fma2(v[4 * h + i], p[i], q[i]);
         }
-        store16<ALIGNED>(f.y + row * f.y_stride + col, col, cols, v, lane > 0, lane < 31);
+        store16<ALIGNED>(f.y + rowStart(row, f.y_stride) + col, col, cols, v, lane > 0, lane < 31);
     }
 }
 
@@ -302,12 +301,12 @@ int thor_b200_layernorm_launch(const thor_b200_layernorm_desc* d, const void* x,
         f.sum = static_cast<T*>(sum);
         f.mean = mean;
         f.rstd = rstd;
-        f.y_stride = d->y_stride;
+        f.y_stride = strideOf(d->y_stride, d->rows);
         f.gamma = paramOf(gamma, d->param_dtype);
         f.beta = paramOf(beta, d->param_dtype);
         f.packable = d->param_dtype == d->dtype;
-        f.kept = Writer{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), codePitch(d->cols), scalePitch(d->cols), d->code_dtype};
-        f.rows = d->rows;
+        f.kept = Writer{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), static_cast<uint32_t>(codePitch(d->cols)), static_cast<uint32_t>(scalePitch(d->cols)), d->code_dtype};
+        f.rows = static_cast<uint32_t>(d->rows);
         f.cols = static_cast<uint32_t>(d->cols);
         f.eps = d->eps;
         f.count = static_cast<float>(d->cols);

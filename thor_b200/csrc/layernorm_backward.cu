@@ -26,22 +26,21 @@ struct Backward {
     const float* rstd;
     Param gamma;
     Reader kept;
-    uint64_t rows;
-    uint32_t cols, team;
+    uint32_t rows, cols, team;
     float inverse;  // 1 / cols
     float* partial;    // [partial rows][2][padded], nullptr: no parameter gradients
     uint32_t padded;
-    uint64_t slab_rows;  // rows of a partial row, in the kernels for long rows
+    uint32_t slab_rows;  // rows of a partial row, in the kernels for long rows
 };
 
 // Normalised values of sixteen columns; what lies past the row's end meets a gradient of zero.
 template <bool KEPT, bool ALIGNED, class T>
 struct Normal {
     Raw<T, ALIGNED> raw;
-    __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetch16(b.x, b.x.p + row * b.x.stride + col, col, cols, raw); }
+    __device__ __forceinline__ void fetch(const Backward<T>& b, uint32_t row, uint32_t col, uint32_t cols) { fetch16(b.x, b.x.p + rowStart(row, b.x.stride) + col, col, cols, raw); }
     template <bool MIXED = false>
-    __device__ __forceinline__ void expand(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols, float mean, float rstd, float2 (&n)[8]) const {
-        expand16<T, ALIGNED, MIXED>(b.x.p + row * b.x.stride + col, col, cols, raw, n);
+    __device__ __forceinline__ void expand(const Backward<T>& b, uint32_t row, uint32_t col, uint32_t cols, float mean, float rstd, float2 (&n)[8]) const {
+        expand16<T, ALIGNED, MIXED>(b.x.p + rowStart(row, b.x.stride) + col, col, cols, raw, n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) n[i] = mul2(add2(n[i], both(-mean)), both(rstd));
     }
@@ -49,9 +48,9 @@ struct Normal {
 template <bool ALIGNED, class T>
 struct Normal<true, ALIGNED, T> {
     RawCodes raw;
-    __device__ __forceinline__ void fetch(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols) { fetchCodes(codesAt(b.kept, row, col), scaleAt(b.kept, row, col), col, cols, raw); }
+    __device__ __forceinline__ void fetch(const Backward<T>& b, uint32_t row, uint32_t col, uint32_t cols) { fetchCodes(codesAt(b.kept, row, col), scaleAt(b.kept, row, col), col, cols, raw); }
     template <bool MIXED = false>
-    __device__ __forceinline__ void expand(const Backward<T>& b, uint64_t, uint32_t col, uint32_t cols, float, float, float2 (&n)[8]) const {
+    __device__ __forceinline__ void expand(const Backward<T>& b, uint32_t, uint32_t col, uint32_t cols, float, float, float2 (&n)[8]) const {
         expandCodes<!ALIGNED>(b.kept.code, col, cols, raw, n);
     }
 };
@@ -73,18 +72,18 @@ __device__ __forceinline__ void weigh16(const Backward<T>& b, uint32_t col, uint
 }
 // rstd * (w - c1 - n c2) [+ grad_sum]
 template <bool ALIGNED, class T>
-__device__ __forceinline__ void finish16(const Backward<T>& b, uint64_t row, uint32_t col, uint32_t cols, float2 (&w)[8], const float2 (&n)[8], float c1, float c2, float rstd,
+__device__ __forceinline__ void finish16(const Backward<T>& b, uint32_t row, uint32_t col, uint32_t cols, float2 (&w)[8], const float2 (&n)[8], float c1, float c2, float rstd,
                                          const Raw<T, ALIGNED>& stream, bool before, bool after) {
     const float2 scale = both(rstd), shift = both(-rstd * c1), slope = both(-rstd * c2);
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = fma2(n[i], slope, fma2(w[i], scale, shift));
     if (b.grad_sum.p != nullptr) {
         float2 r[8];
-        expand16(b.grad_sum.p + row * b.grad_sum.stride + col, col, cols, stream, r);
+        expand16(b.grad_sum.p + rowStart(row, b.grad_sum.stride) + col, col, cols, stream, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = add2(w[i], r[i]);
     }
-    store16<ALIGNED>(b.grad_input + row * b.cols + col, col, cols, w, before, after);
+    store16<ALIGNED>(b.grad_input + rowStart(row, b.cols) + col, col, cols, w, before, after);
 }
 
 template <class T, bool KEPT, bool ALIGNED>
@@ -107,7 +106,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
     auto fetch = [&](uint32_t r) {
         const bool there = r < b.rows;
         cols = there ? b.cols : 0;
-        fetch16(b.grad, b.grad.p + static_cast<uint64_t>(r) * b.grad.stride + col, col, cols, grad);
+        fetch16(b.grad, b.grad.p + rowStart(r, b.grad.stride) + col, col, cols, grad);
         normal.fetch(b, r, col, cols);
         rstd = there ? __ldg(b.rstd + r) : 0.0f;
         if constexpr (!KEPT) mean = there ? __ldg(b.mean + r) : 0.0f;
@@ -122,13 +121,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
     // the same number of turns for the whole CTA; a team without a row has cols = 0
     for (uint32_t base = blockIdx.x * teams; base < b.rows; base += step, row += step) {
         float2 w[8], n[8];
-        expand16(b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col, col, cols, grad, w);
+        expand16(b.grad.p + rowStart(row, b.grad.stride) + col, col, cols, grad, w);
         normal.expand(b, row, col, cols, mean, rstd, n);
         const uint32_t now_cols = cols;
         const float now_rstd = rstd;
         if constexpr (kAhead) fetch(row + step);
         Raw<T, ALIGNED> stream;
-        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + static_cast<uint64_t>(row) * b.grad_sum.stride + col, col, now_cols, stream);
+        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + rowStart(row, b.grad_sum.stride) + col, col, now_cols, stream);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             dg[i] = fma2(w[i], n[i], dg[i]);
@@ -202,7 +201,7 @@ __device__ __forceinline__ void columnStrip(const Backward<T>& b, uint32_t strip
         for (int k = 0; k < kRows; ++k) {
             const uint32_t row = first + k * step;
             const bool there = row < b.rows;
-            fetch16(b.grad, b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col, col, there ? b.cols : 0, grad[k]);
+            fetch16(b.grad, b.grad.p + rowStart(row, b.grad.stride) + col, col, there ? b.cols : 0, grad[k]);
             normal[k].fetch(b, row, col, there ? b.cols : 0);
             mean[k] = KEPT || !there ? 0.0f : b.mean[row];
             rstd[k] = KEPT || !there ? 0.0f : b.rstd[row];
@@ -211,7 +210,7 @@ __device__ __forceinline__ void columnStrip(const Backward<T>& b, uint32_t strip
         for (int k = 0; k < kRows; ++k) {
             const uint32_t row = first + k * step, cols = row < b.rows ? b.cols : 0;
             float2 d[8], n[8];
-            expand16<T, ALIGNED, true>(b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col, col, cols, grad[k], d);
+            expand16<T, ALIGNED, true>(b.grad.p + rowStart(row, b.grad.stride) + col, col, cols, grad[k], d);
             normal[k].template expand<true>(b, row, col, cols, mean[k], rstd[k], n);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -265,10 +264,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardFewRowsKernel(const __
         const uint32_t row = base + team_id, cols = row < b.rows ? b.cols : 0;
         Raw<T, ALIGNED> grad, stream;
         Normal<KEPT, ALIGNED, T> normal;
-        const T* const grad_at = b.grad.p + static_cast<uint64_t>(row) * b.grad.stride + col;
+        const T* const grad_at = b.grad.p + rowStart(row, b.grad.stride) + col;
         fetch16(b.grad, grad_at, col, cols, grad);
         normal.fetch(b, row, col, cols);
-        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + static_cast<uint64_t>(row) * b.grad_sum.stride + col, col, cols, stream);
+        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + rowStart(row, b.grad_sum.stride) + col, col, cols, stream);
         const float rstd = cols > 0 ? b.rstd[row] : 0.0f, mean = cols > 0 && !KEPT ? b.mean[row] : 0.0f;
         float2 w[8], n[8], s1 = both(0.0f), s2 = both(0.0f);
         expand16(grad_at, col, cols, grad, w);
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(512) gradInputLoopKernel(const __grid_constant
     __shared__ float scratch[2][32];
     gridDependencyWait();
     gridLaunchDependents();
-    const uint64_t row = blockIdx.x;
+    const uint32_t row = blockIdx.x;
     const uint32_t lane = threadIdx.x % 32, step = blockDim.x * kVec;
     const float rstd = b.rstd[row];
     const float mean = KEPT ? 0.0f : b.mean[row];
@@ -297,7 +296,7 @@ __global__ void __launch_bounds__(512) gradInputLoopKernel(const __grid_constant
     for (uint64_t at = threadIdx.x * kVec; at < b.cols; at += step) {
         const uint32_t col = static_cast<uint32_t>(at);
         normal.fetch(b, row, col, b.cols);
-        load16<ALIGNED>(b.grad, b.grad.p + row * b.grad.stride + col, col, b.cols, w);
+        load16<ALIGNED>(b.grad, b.grad.p + rowStart(row, b.grad.stride) + col, col, b.cols, w);
         normal.expand(b, row, col, b.cols, mean, rstd, n);
         float2 p1 = both(0.0f), p2 = both(0.0f);
         weigh16(b, col, b.cols, w, n, p1, p2);
@@ -311,9 +310,9 @@ __global__ void __launch_bounds__(512) gradInputLoopKernel(const __grid_constant
         const uint64_t at = base + threadIdx.x * kVec;
         const uint32_t col = static_cast<uint32_t>(at), cols = at < b.cols ? b.cols : 0;
         Raw<T, ALIGNED> stream;
-        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + row * b.grad_sum.stride + col, col, cols, stream);
+        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + rowStart(row, b.grad_sum.stride) + col, col, cols, stream);
         normal.fetch(b, row, col, cols);
-        load16<ALIGNED>(b.grad, b.grad.p + row * b.grad.stride + col, col, cols, w);
+        load16<ALIGNED>(b.grad, b.grad.p + rowStart(row, b.grad.stride) + col, col, cols, w);
         normal.expand(b, row, col, cols, mean, rstd, n);
         float2 p1 = both(0.0f), p2 = both(0.0f);
         weigh16(b, col, cols, w, n, p1, p2);
@@ -329,14 +328,14 @@ __global__ void __launch_bounds__(256) columnSumKernel(const __grid_constant__ B
     gridLaunchDependents();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t first = blockIdx.x * 512, col = first + lane * kVec;
-    const uint64_t end = min(b.rows, (blockIdx.y + 1) * b.slab_rows);
+    const uint32_t end = min(b.rows, (blockIdx.y + 1) * b.slab_rows);
     float2 dg[8], db[8], d[8], n[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) dg[i] = db[i] = both(0.0f);
-    for (uint64_t row = blockIdx.y * b.slab_rows + warp; row < end; row += 8) {
+    for (uint32_t row = blockIdx.y * b.slab_rows + warp; row < end; row += 8) {
         Normal<KEPT, ALIGNED, T> normal;
         normal.fetch(b, row, col, b.cols);
-        load16<ALIGNED>(b.grad, b.grad.p + row * b.grad.stride + col, col, b.cols, d);
+        load16<ALIGNED>(b.grad, b.grad.p + rowStart(row, b.grad.stride) + col, col, b.cols, d);
         normal.expand(b, row, col, b.cols, KEPT ? 0.0f : b.mean[row], KEPT ? 0.0f : b.rstd[row], n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -531,14 +530,14 @@ int thor_b200_layernorm_backward_launch(const thor_b200_layernorm_desc* d, const
         b.mean = mean;
         b.rstd = rstd;
         b.gamma = paramOf(gamma, d->param_dtype);
-        b.kept = Reader{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), codePitch(d->cols), scalePitch(d->cols), d->code_dtype};
-        b.rows = d->rows;
+        b.kept = Reader{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<uint32_t>(codePitch(d->cols)), static_cast<uint32_t>(scalePitch(d->cols)), d->code_dtype};
+        b.rows = static_cast<uint32_t>(d->rows);
         b.cols = static_cast<uint32_t>(d->cols);
         b.team = p.team;
         b.inverse = 1.0f / static_cast<float>(d->cols);
         b.partial = params ? static_cast<float*>(workspace) : nullptr;
         b.padded = p.padded;
-        b.slab_rows = p.slab_rows;
+        b.slab_rows = static_cast<uint32_t>(p.slab_rows);
         return launchBackward<T>(b, p, aligned, d->grad_param_dtype, grad_gamma, grad_beta, stream);
     });
 }

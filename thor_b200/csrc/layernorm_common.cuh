@@ -205,10 +205,7 @@ inline int checkDesc(const char* who, const thor_b200_layernorm_desc* d) {
     TB_REQUIRE(d->eps >= 0.0f, "%s: eps must not be negative", who);
     return THOR_B200_OK;
 }
-inline int checkStride(const char* who, const char* what, int64_t stride, const thor_b200_layernorm_desc& d) {
-    TB_REQUIRE(d.rows <= 1 || (stride >= 0 && static_cast<uint64_t>(stride) >= d.cols), "%s: the row stride of %s is smaller than a row", who, what);
-    return THOR_B200_OK;
-}
+inline int checkStride(const char* who, const char* what, int64_t stride, const thor_b200_layernorm_desc& d) { return checkRowStride(who, what, stride, d.rows, d.cols); }
 // A tensor that may be absent.
 inline int checkPointer(const char* who, const void* p, size_t alignment) {
     TB_REQUIRE(isAligned(p, alignment), "%s: a tensor pointer is not aligned to its elements", who);
