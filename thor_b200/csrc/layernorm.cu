@@ -59,7 +59,8 @@ __device__ __forceinline__ float centre16(float2 (&v)[8], float mean, uint32_t c
     return s.x + s.y;
 }
 
-template <class T, int CHUNKS, bool PACKED, bool ALIGNED, bool RESIDUAL>
+// GROUP: teams of up to 32 lanes; otherwise of whole warps.
+template <class T, int CHUNKS, bool GROUP, bool PACKED, bool ALIGNED, bool RESIDUAL>
 __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKernel(const __grid_constant__ Forward<T> f) {
     constexpr bool kAhead = ALIGNED && !RESIDUAL;  // the next row is loaded while this one is worked on
     __shared__ Scratch scratch;
@@ -69,14 +70,14 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
     gridLaunchDependents();
     const uint32_t team = f.team, team_id = threadIdx.x / team, t = threadIdx.x - team_id * team, teams = blockDim.x / team;
     const uint32_t lane = threadIdx.x % 32, chunks = CHUNKS * team;
-    const bool before = team < 32 ? t > 0 : lane > 0, after = team < 32 ? t + 1 < team : lane < 31;
+    const bool before = GROUP ? t > 0 : lane > 0, after = GROUP ? t + 1 < team : lane < 31;
     const uint32_t step = gridDim.x * teams;
     // columns of this warp, and of the warp whose results this lane fetches
-    const uint32_t warps = team <= 32 ? 1 : team / 32, my_warp = threadIdx.x / 32 - team_id * warps;
-    const float own_count = team <= 32 ? f.count : warpColumns(my_warp, team, f.cols, CHUNKS);
-    const float its_count = lane % 16 < warps ? (team <= 32 ? f.count : warpColumns(lane % 16, team, f.cols, CHUNKS)) : 0.0f;
+    const uint32_t warps = GROUP ? 1 : team / 32, my_warp = GROUP ? 0 : threadIdx.x / 32 - team_id * warps;
+    const float own_count = GROUP ? f.count : warpColumns(my_warp, team, f.cols, CHUNKS);
+    const float its_count = GROUP || lane % 16 >= warps ? 0.0f : warpColumns(lane % 16, team, f.cols, CHUNKS);
     const float own_inverse = own_count > 0.0f ? 1.0f / own_count : 0.0f, its_inverse = its_count > 0.0f ? 1.0f / its_count : 0.0f;
-    const uint32_t span = team < 32 ? team : 32;  // lanes that share a row
+    const uint32_t span = GROUP ? team : 32;  // lanes that share a row
     int slot = 0;
     uint32_t row = blockIdx.x * teams + team_id;
     uint32_t cols = row < f.rows ? f.cols : 0;
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
         for (int k = 0; k < CHUNKS; ++k) m2 += centre16<ALIGNED>(v[k], mean, (t + k * team) * kVec, cols);
         m2 = laneSum(m2, span);
         float shift = 0.0f;  // from the warp's mean to the row's
-        if (team > 32) {
+        if constexpr (!GROUP) {
             if (lane == 0) scratch.part[slot][team_id][my_warp] = make_float2(s, m2);
             asm volatile("bar.sync %0, %1;" ::"r"(team_id + 1), "r"(team) : "memory");
             const float2 its = lane % 16 < warps ? scratch.part[slot][team_id][lane % 16] : make_float2(0.0f, 0.0f);
@@ -248,15 +249,17 @@ int launchForward(const Forward<T>& given, bool aligned, cudaStream_t stream) {
         const size_t shared = (packed ? 4 : 8) * sizeof(uint4) * per_thread * f.team;
         return byFlag(f.residual.p != nullptr, [&](auto residual) {
             constexpr bool R = decltype(residual)::value;
-            auto launch = [&](auto chunks_a_thread, auto in_own_type) {
-                constexpr auto kernel = &forwardKernel<T, decltype(chunks_a_thread)::value, decltype(in_own_type)::value, A, R>;
+            auto launch = [&](auto chunks_a_thread, auto group, auto in_own_type) {
+                constexpr auto kernel = &forwardKernel<T, decltype(chunks_a_thread)::value, decltype(group)::value, decltype(in_own_type)::value, A, R>;
                 if (int st = allowShared<kernel>(shared)) return st;
                 TB_CUDA(launchDependent(kernel, grid, block, shared, stream, f));
                 countLaunch();
                 return static_cast<int>(THOR_B200_OK);
             };
             auto launchFor = [&](auto in_own_type) {
-                return per_thread == 1 ? launch(std::integral_constant<int, 1>{}, in_own_type) : launch(std::integral_constant<int, 2>{}, in_own_type);
+                if (f.team <= 32) return launch(std::integral_constant<int, 1>{}, std::true_type{}, in_own_type);
+                if (per_thread == 1) return launch(std::integral_constant<int, 1>{}, std::false_type{}, in_own_type);
+                return launch(std::integral_constant<int, 2>{}, std::false_type{}, in_own_type);
             };
             if constexpr (sizeof(T) == 2)
                 if (packed) return launchFor(std::true_type{});
