@@ -88,7 +88,8 @@ __device__ __forceinline__ void finish16(const Backward<T>& b, uint32_t row, uin
 
 // Asks L2 for the row that a team takes kRowsAhead turns from now.  A register load one turn ahead hides L2's latency, not that of the memory behind it:
 // [32768, 8192] bf16 from a checkpoint 266 us without, 248 with it; from the saved input 278 and 249.  Three or five turns ahead are no better
-// than two, requests of rows shorter than 512 columns cost more than they give.
+// than two.  Teams of fewer than 64 threads do not ask, nor of fewer than 128 where the input was saved or the width is odd: there the
+// requests cost more than they give ([65536, 1024] fp32 131 us with, 127 without).
 constexpr uint32_t kRowsAhead = 2;
 template <bool ALIGNED>
 __device__ __forceinline__ void requestBytes(const void* from, uint32_t bytes) {
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
     Params::stage(b.gamma, 1.0f, shared, team, b.cols);
     __syncthreads();
     int slot = 0;
-    const bool asks = team > 32 && t == 0;
+    const bool asks = team >= (KEPT && ALIGNED ? 64 : 128) && t == 0;
     // the same number of turns for the whole CTA; a team without a row has cols = 0
     for (uint32_t base = blockIdx.x * teams; base < b.rows; base += step, row += step) {
         float2 w[8], n[8];
