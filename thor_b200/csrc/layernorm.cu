@@ -34,28 +34,21 @@ struct Forward {
     float eps, count, inverse;  // count = cols, inverse = 1 / cols
 };
 
-// v - mean, zero past the row's end, and the sum of the squares
+// v - mean, zero past the row's end
 template <bool ALIGNED>
-__device__ __forceinline__ float centre16(float2 (&v)[8], float mean, uint32_t col, uint32_t cols) {
-    float2 s = both(0.0f);
-    if (col < cols) {
+__device__ __forceinline__ void centre16(const float2 (&v)[8], float mean, uint32_t col, uint32_t cols, float2 (&d)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = add2(v[i], both(-mean));
-        if (!ALIGNED && col + 16 > cols) {
+    for (int i = 0; i < 8; ++i) d[i] = col < cols ? add2(v[i], both(-mean)) : both(0.0f);
+    if constexpr (!ALIGNED) cutRow(col, cols, d);
+}
+__device__ __forceinline__ float squares16(const float2 (&d)[8]) {
+    float2 s = mul2(d[0], d[0]), u = mul2(d[1], d[1]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (col + 2 * i >= cols) v[i].x = 0.0f;
-                if (col + 2 * i + 1 >= cols) v[i].y = 0.0f;
-            }
-        }
-        float2 u = both(0.0f);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            s = fma2(v[i], v[i], s);
-            u = fma2(v[i + 1], v[i + 1], u);
-        }
-        s = add2(s, u);
+    for (int i = 2; i < 8; i += 2) {
+        s = fma2(d[i], d[i], s);
+        u = fma2(d[i + 1], d[i + 1], u);
     }
+    s = add2(s, u);
     return s.x + s.y;
 }
 
@@ -124,9 +117,12 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
         s = laneSum(s, span);
         float mean = divideBy(s, own_count, own_inverse), m2 = 0.0f;  // of the warp's columns
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) m2 += centre16<ALIGNED>(v[k], mean, (t + k * team) * kVec, cols);
+        for (int k = 0; k < CHUNKS; ++k) {
+            float2 d[8];
+            centre16<ALIGNED>(v[k], mean, (t + k * team) * kVec, cols, d);
+            m2 += squares16(d);
+        }
         m2 = laneSum(m2, span);
-        float shift = 0.0f;  // from the warp's mean to the row's
         if constexpr (!GROUP) {
             if (lane == 0) scratch.part[slot][team_id][my_warp] = make_float2(s, m2);
             asm volatile("bar.sync %0, %1;" ::"r"(team_id + 1), "r"(team) : "memory");
@@ -135,7 +131,6 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
             const float row_mean = divideBy(laneSum(its.x, 16), f.count, f.inverse);
             const float off = its_count > 0.0f ? divideBy(its.x, its_count, its_inverse) - row_mean : 0.0f;
             m2 = laneSum(fmaf(its_count * off, off, its.y), 16);
-            shift = mean - row_mean;
             mean = row_mean;
         }
         const float rstd = inverseRoot(divideBy(m2, f.count, f.inverse) + f.eps);
@@ -146,9 +141,9 @@ __global__ void __launch_bounds__(kMaxThreads, residentCtas(CHUNKS)) forwardKern
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
             const uint32_t col = (t + k * team) * kVec;
+            centre16<ALIGNED>(v[k], mean, col, cols, v[k]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[k][i] = fma2(v[k][i], both(rstd), both(shift * rstd));
-            if constexpr (!ALIGNED) cutRow(col, cols, v[k]);
+            for (int i = 0; i < 8; ++i) v[k][i] = mul2(v[k][i], both(rstd));
             if (f.kept.codes != nullptr) writeCodes(codesAt(f.kept, row, col), scaleAt(f.kept, row, col), f.kept.code, col, cols, v[k]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -199,7 +194,8 @@ __global__ void __launch_bounds__(512) forwardLoopKernel(const __grid_constant__
     s = 0.0f;
     for (uint64_t at = threadIdx.x * kVec; at < f.cols; at += step) {
         input16<ALIGNED>(f, row, static_cast<uint32_t>(at), f.cols, v);
-        s += centre16<ALIGNED>(v, mean, static_cast<uint32_t>(at), f.cols);
+        centre16<ALIGNED>(v, mean, static_cast<uint32_t>(at), f.cols, v);
+        s += squares16(v);
     }
     const float rstd = inverseRoot(divideBy(ctaSum(s, scratch[1]), f.count, f.inverse) + f.eps);
     if (threadIdx.x == 0) {
@@ -210,7 +206,7 @@ __global__ void __launch_bounds__(512) forwardLoopKernel(const __grid_constant__
         const uint64_t at = base + threadIdx.x * kVec;
         const uint32_t col = static_cast<uint32_t>(at), cols = at < f.cols ? f.cols : 0;
         input16<ALIGNED>(f, row, col, cols, v);
-        centre16<ALIGNED>(v, mean, col, cols);
+        centre16<ALIGNED>(v, mean, col, cols, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], both(rstd));
         if (f.kept.codes != nullptr) writeCodes(codesAt(f.kept, row, col), scaleAt(f.kept, row, col), f.kept.code, col, cols, v);
