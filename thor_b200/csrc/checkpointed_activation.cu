@@ -16,8 +16,8 @@ using namespace ck8;
 // exponential is below the smallest normal number.  The form keeps the relative accuracy of the far tail, and the exponential is the one
 // that the derivative needs.  Degree 9: 2.1e-7 of the value as evaluated in fp32 (fp32 tensors); degree 6: 4.8e-6, a hundredth of
 // half a unit of fp16 (16-bit tensors), three instructions a pair less.  For fp32 the rounding of x^2 is carried into the exponent.
-// Two elements an instruction (f32x2) and one exponential and one reciprocal an element; the toolkit's erfcf and expf made the backward kernel
-// wait for the arithmetic pipes (GELU [2999, 11001] fp16: 112 us).
+// Two elements an instruction (f32x2) and one exponential and one reciprocal an element; with the toolkit's erfcf and expf the backward kernel
+// waited for the arithmetic pipes.
 template <int KIND, bool FULL>
 __device__ __forceinline__ void activation2(float2 x, float2& value, float2& slope) {
     if constexpr (KIND == THOR_B200_ACTIVATION_SWISH) {
@@ -63,8 +63,17 @@ __device__ __forceinline__ void activation2(float2 x, float2& value, float2& slo
     }
 }
 
+// CTAs of 256 threads that an SM shall hold, which caps the registers (left alone the compiler takes 56 to 80 and too few warps are there to wait with).
+// GELU backward [8192, 8192] bf16: 76.1 us uncapped, 57.2 with five, 52.9 with six; gated Swish backward 90.4, 80.8, 81.6.  Odd rows of fp32
+// spill under any cap.
+template <class T, bool GATED, bool ALIGNED, bool BACKWARD>
+constexpr int residentCtas() {
+    if (sizeof(T) == 4) return ALIGNED || (!GATED && !BACKWARD) ? 5 : 1;
+    return GATED || (BACKWARD && !ALIGNED) ? 5 : 6;
+}
+
 template <class T, int KIND, bool GATED, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) activationKernel(Rows<T> x, Rows<T> gate, T* __restrict__ y, uint32_t y_stride, Writer out, Writer gate_out, Walk w) {
+__global__ void __launch_bounds__(kThreads, residentCtas<T, GATED, ALIGNED, false>()) activationKernel(Rows<T> x, Rows<T> gate, T* __restrict__ y, uint32_t y_stride, Writer out, Writer gate_out, Walk w) {
     gridDependencyWait();
     gridLaunchDependents();
     uint32_t row, col, cols;
@@ -93,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) activationKernel(Rows<T> x, Rows<T> 
 }
 
 template <class T, int KIND, bool GATED, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) activationBackwardKernel(Rows<T> grad, Reader in, Reader gate_in, T* __restrict__ grad_x, uint32_t grad_x_stride,
+__global__ void __launch_bounds__(kThreads, residentCtas<T, GATED, ALIGNED, true>()) activationBackwardKernel(Rows<T> grad, Reader in, Reader gate_in, T* __restrict__ grad_x, uint32_t grad_x_stride,
                                                                      T* __restrict__ grad_gate, uint32_t grad_gate_stride, Walk w) {
     gridDependencyWait();
     gridLaunchDependents();
