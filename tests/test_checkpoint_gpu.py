@@ -182,6 +182,13 @@ def test_no_rows():
     assert (ck.rows, ck.cols) == (0, 64) and CheckpointUnpack().stamp(ck).run().shape == (0, 64)
 
 
+def test_row_strides_past_32_bits_are_refused():
+    x = torch.empty((1 << 32) + 16, dtype=torch.float16, device="cuda")
+    with pytest.raises(ThorB200InvalidArgument, match="2\\^32 elements between rows"):
+        CheckpointPack().stamp(x.as_strided((2, 16), (1 << 32, 1)))
+    CheckpointPack().stamp(x.as_strided((2, 16), ((1 << 32) - 1, 1)))
+
+
 def test_refusals():
     x = torch.randn(8, 64, device="cuda")
     ck = CheckpointPack().stamp(x).checkpoint

@@ -134,6 +134,40 @@ def test_many_rows_and_their_column_sums():
         assert all(torch.equal(a, b) for a, b in zip(first, (plan.grad_input, plan.grad_gamma, plan.grad_beta)))  # a fixed order
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(513, 16), (1201, 33), (613, 500), (2001, 1024), (700, 1032), (601, 3008), (513, 4095), (519, 4112), (741, 5001), (741, 5120), (889, 6144), (520, 6160),
+                                       (513, 8191), (600, 8192), (513, 8208), (515, 9001)])
+@pytest.mark.parametrize("source", ["x", "e4m3", "e5m2"])
+def test_backward_of_many_rows(rows, cols, dtype, source):
+    """More rows than one launch takes: teams that walk several rows one at a time or two at once, with a last turn that not every team has a row
+    for, partial rows and their fold.  A column's sum is a chain of at most 2001 / 148 + 512 / 2 teams + 148 / 8 + 8 additions: below 512."""
+    x, r, gamma, beta = tensors(rows, cols, dtype, torch.float32, 5)
+    grad = tensors(rows, cols, dtype, torch.float32, 6)[1]
+    forward = LayerNorm(1e-5, {"x": None, "e4m3": DataType.fp8_e4m3, "e5m2": DataType.fp8_e5m2}[source]).stamp(x, gamma, beta)
+    forward.run()
+    rstd = forward.rstd.double()
+    if source == "x":
+        n = (x.double() - forward.mean.double()[:, None]) * rstd[:, None]
+        slip = 2 * F32 * n.abs() + F32 * (x.double().abs() + forward.mean.double().abs()[:, None]) * rstd[:, None]
+        kept = dict(x=x, mean=forward.mean)
+    else:
+        n = unpack64(forward.checkpoint.codes, forward.checkpoint.scales, cols)
+        slip = torch.zeros_like(n)
+        kept = dict(checkpoint=forward.checkpoint)
+    g = grad.double()
+    dx, dg, db = layernorm_grads64(g, n, rstd, gamma.double())
+    w = g * gamma.double()
+    row1, row2 = w.abs().mean(1, keepdim=True), (w * n).abs().mean(1, keepdim=True)
+    error = rstd[:, None] * (D * F32 * (row1 + n.abs() * row2) + n.abs() * (w.abs() * slip).mean(1, keepdim=True) + slip * row2 + 8 * F32 * (w.abs() + row1 + n.abs() * row2))
+    for grad_sum in (None, r):
+        plan = LayerNormBackward().stamp(grad, forward.rstd, gamma=gamma, grad_sum=grad_sum, **kept)
+        plan.run()
+        want = dx if grad_sum is None else dx + r.double()
+        assert ((plan.grad_input.double() - want).abs() <= error + 4 * F32 * want.abs() + HALF_ULP[dtype] * 1.01 * want.abs() + TINY[dtype]).all()
+        for got, exact, size, extra in ((plan.grad_gamma, dg, (g * n).abs().sum(0), (g.abs() * slip).sum(0)), (plan.grad_beta, db, g.abs().sum(0), 0.0)):
+            assert ((got.double() - exact).abs() <= (D + 2) * F32 * size + extra + F32 * exact.abs()).all()
+
+
 def test_gradients_against_differences():
     """sum(c * layernorm(x)) by central differences of the 64-bit function, in x, gamma and beta."""
     rows, cols, eps = 3, 40, 1e-5

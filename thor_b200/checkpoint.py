@@ -2,7 +2,8 @@
 
 An operator is described once, stamped on its tensors (checks, output allocation) and run as often as the step repeats; run()
 is one call into the library on the stream given at stamp time or, without one, on the current stream, and allocates nothing, so it can be
-captured into a CUDA graph."""
+captured into a CUDA graph.  A stamped operator owns its outputs and workspace: two runs of one plan (direct or as replays of graphs that hold
+it) must not overlap in time, and a plan must outlive the work and the graphs that use it; plans of the same operator are independent of one another."""
 from __future__ import annotations
 
 import ctypes as C
@@ -40,7 +41,7 @@ def as_rows(t: torch.Tensor, what: str) -> tuple[int, int, int]:
     """(rows, cols, elements between rows) of a CUDA tensor whose last axis is dense and whose leading axes are one evenly spaced run of rows."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         refuse(f"{what} must be a CUDA tensor (no CPU path in this library)")
-    if from_torch(t.dtype) not in VALUE_DTYPES if t.dtype in (torch.float32, torch.float16, torch.bfloat16) else True:
+    if t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         refuse(f"{what} must be fp32, fp16 or bf16, got {t.dtype}")
     if t.dim() == 0 or t.shape[-1] == 0:
         refuse(f"{what} needs a last axis of at least one column")
@@ -57,6 +58,8 @@ def as_rows(t: torch.Tensor, what: str) -> tuple[int, int, int]:
     stride = lead[-1][1] if lead else cols
     if rows > 1 and stride < cols:
         refuse(f"{what}: rows overlap (row stride {stride}, {cols} columns)")
+    if cols >= 1 << 31 or rows >= 1 << 32 or (rows > 1 and stride >= 1 << 32):
+        refuse(f"{what}: fewer than 2^31 columns, 2^32 rows and 2^32 elements between rows are taken")
     return rows, cols, stride
 
 
@@ -228,8 +231,9 @@ class StampedCheckpointUnpack(Stamped):
 
 
 class CheckpointUnpack:
-    """Writes the values that a checkpoint stands for as fp32, fp16 or bf16 (bf16 and fp32 hold every finite one of them exactly, apart
-    from the ends of the range; fp16 rounds once)."""
+    """Writes the values that a checkpoint stands for as fp32, fp16 or bf16 (bf16 and fp32 hold every one of them exactly down to
+    their subnormal numbers; a code that stands for 2^128, half a step above the largest numbers, unpacks as infinity.  fp16 rounds once, and values
+    from 65520 on are infinite there)."""
 
     def __init__(self, dtype: DataType = DataType.bf16):
         self.dtype = DataType(dtype)

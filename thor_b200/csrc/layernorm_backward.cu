@@ -110,8 +110,14 @@ __device__ __forceinline__ void requestRow(const Backward<T>& b, uint32_t row) {
     else requestBytes<ALIGNED>(b.x.p + rowStart(row, b.x.stride), b.cols * static_cast<uint32_t>(sizeof(T)));
 }
 
-template <class T, bool KEPT, bool ALIGNED>
-__global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_constant__ Backward<T> b) {
+// Teams that leave a quarter of the threads unused or more (a width of 5120 makes one of 320) work on two rows at once, with the registers that are left
+// over: twice the arithmetic between two barriers.  [32768, 5120] bf16 from a checkpoint 202 -> 167 us, [32768, 6144] 214 -> 183, [65536, 3008] 211 -> 179.
+// From the saved input (194 -> 206 us) and with odd rows (333 -> 404) two rows do not fit the registers, nor in fp32.
+constexpr uint32_t kPairThreads = 384;
+
+// ROWS: rows that a team works on at once.
+template <class T, int ROWS, bool KEPT, bool ALIGNED>
+__global__ void __launch_bounds__(ROWS == 2 ? kPairThreads : kMaxThreads, 1) backwardKernel(const __grid_constant__ Backward<T> b) {
     // the next row is loaded while this one is worked on; odd rows of fp32 have no registers for it ([32768, 5001] bf16 405 -> 333 us)
     constexpr bool kAhead = ALIGNED || sizeof(T) == 2;
     __shared__ Scratch scratch;
@@ -124,17 +130,21 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
     const bool before = team < 32 ? t > 0 : lane > 0, after = team < 32 ? t + 1 < team : lane < 31;
     const uint32_t step = gridDim.x * teams;
     uint32_t row = blockIdx.x * teams + team_id;
-    Raw<T, ALIGNED> grad;
-    Normal<KEPT, ALIGNED, T> normal;
-    float rstd = 0.0f, mean = 0.0f;
-    uint32_t cols = 0;
-    auto fetch = [&](uint32_t r) {
-        const bool there = r < b.rows;
-        cols = there ? b.cols : 0;
-        fetch16(b.grad, b.grad.p + rowStart(r, b.grad.stride) + col, col, cols, grad);
-        normal.fetch(b, r, col, cols);
-        rstd = there ? __ldg(b.rstd + r) : 0.0f;
-        if constexpr (!KEPT) mean = there ? __ldg(b.mean + r) : 0.0f;
+    Raw<T, ALIGNED> grad[ROWS];
+    Normal<KEPT, ALIGNED, T> normal[ROWS];
+    float rstd[ROWS], mean[ROWS];
+    uint32_t cols[ROWS];
+    auto fetch = [&](uint32_t first) {
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const uint32_t r = first + k * step;
+            const bool there = r < b.rows;
+            cols[k] = there ? b.cols : 0;
+            fetch16(b.grad, b.grad.p + rowStart(r, b.grad.stride) + col, col, cols[k], grad[k]);
+            normal[k].fetch(b, r, col, cols[k]);
+            rstd[k] = there ? __ldg(b.rstd + r) : 0.0f;
+            mean[k] = !KEPT && there ? __ldg(b.mean + r) : 0.0f;
+        }
     };
     float2 dg[8], db[8];
 #pragma unroll
@@ -145,37 +155,58 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backwardKernel(const __grid_co
     int slot = 0;
     const bool asks = team >= (KEPT && ALIGNED ? 64 : 128) && t == 0;
     // the same number of turns for the whole CTA; a team without a row has cols = 0
-    for (uint32_t base = blockIdx.x * teams; base < b.rows; base += step, row += step) {
-        float2 w[8], n[8];
-        expand16(b.grad.p + rowStart(row, b.grad.stride) + col, col, cols, grad, w);
-        normal.expand(b, row, col, cols, mean, rstd, n);
-        const uint32_t now_cols = cols;
-        const float now_rstd = rstd;
-        if (asks) requestRow<T, ALIGNED>(b, row + kRowsAhead * step);
-        if constexpr (kAhead) fetch(row + step);
-        Raw<T, ALIGNED> stream;
-        if (b.grad_sum.p != nullptr) fetch16(b.grad_sum, b.grad_sum.p + rowStart(row, b.grad_sum.stride) + col, col, now_cols, stream);
+    for (uint32_t base = blockIdx.x * teams; base < b.rows; base += ROWS * step, row += ROWS * step) {
+        float2 w[ROWS][8], n[ROWS][8], sums[ROWS];
+        uint32_t now_cols[ROWS];
+        float now_rstd[ROWS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            dg[i] = fma2(w[i], n[i], dg[i]);
-            db[i] = add2(db[i], w[i]);
+        for (int k = 0; k < ROWS; ++k) {
+            expand16(b.grad.p + rowStart(row + k * step, b.grad.stride) + col, col, cols[k], grad[k], w[k]);
+            normal[k].expand(b, row + k * step, col, cols[k], mean[k], rstd[k], n[k]);
+            now_cols[k] = cols[k];
+            now_rstd[k] = rstd[k];
+            if (asks) requestRow<T, ALIGNED>(b, row + (kRowsAhead * ROWS + k) * step);
         }
-        float2 s1 = both(0.0f), s2 = both(0.0f);
+        if constexpr (kAhead) fetch(row + ROWS * step);
+        Raw<T, ALIGNED> stream[ROWS];
+        if (b.grad_sum.p != nullptr) {
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k)
+                fetch16(b.grad_sum, b.grad_sum.p + rowStart(row + k * step, b.grad_sum.stride) + col, col, now_cols[k], stream[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                dg[i] = fma2(w[k][i], n[k][i], dg[i]);
+                db[i] = add2(db[i], w[k][i]);
+            }
+        }
+        float2 s1[ROWS], s2[ROWS];
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) s1[k] = s2[k] = both(0.0f);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float2 g[4];
             Params::read(shared, team, t, h, g);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[4 * h + i] = mul2(w[4 * h + i], g[i]);
-                s1 = add2(s1, w[4 * h + i]);
-                s2 = fma2(w[4 * h + i], n[4 * h + i], s2);
+            for (int k = 0; k < ROWS; ++k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[k][4 * h + i] = mul2(w[k][4 * h + i], g[i]);
+                    s1[k] = add2(s1[k], w[k][4 * h + i]);
+                    s2[k] = fma2(w[k][4 * h + i], n[k][4 * h + i], s2[k]);
+                }
             }
         }
-        const float2 s = teamSum(make_float2(s1.x + s1.y, s2.x + s2.y), team, team_id, scratch, slot);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) sums[k] = make_float2(s1[k].x + s1[k].y, s2[k].x + s2[k].y);
+        teamSums(sums, team, team_id, scratch, slot);
         slot ^= 1;
-        finish16<ALIGNED>(b, row, col, now_cols, w, n, s.x * b.inverse, s.y * b.inverse, now_rstd, stream, before, after);
-        if constexpr (!kAhead) fetch(row + step);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k)
+            finish16<ALIGNED>(b, row + k * step, col, now_cols[k], w[k], n[k], sums[k].x * b.inverse, sums[k].y * b.inverse, now_rstd[k], stream[k], before, after);
+        if constexpr (!kAhead) fetch(row + ROWS * step);
     }
     if (b.partial == nullptr) return;
     // A partial row keeps the threads' order: value i of thread t at i * team + t.
@@ -468,7 +499,15 @@ int launchBackward(const Backward<T>& b, const Plan& p, bool aligned, int grad_p
                 return static_cast<int>(THOR_B200_OK);
             }
             if (p.fused) {
-                TB_CUDA(launchDependent(backwardKernel<T, K, A>, dim3(p.partial_rows), dim3(p.team * p.teams), 0, stream, b));
+                const uint32_t threads = p.team * p.teams;
+                if constexpr (sizeof(T) == 2 && A && K) {
+                    if (threads <= kPairThreads) {
+                        TB_CUDA(launchDependent(backwardKernel<T, 2, K, A>, dim3(p.partial_rows), dim3(threads), 0, stream, b));
+                        countLaunch();
+                        return static_cast<int>(THOR_B200_OK);
+                    }
+                }
+                TB_CUDA(launchDependent(backwardKernel<T, 1, K, A>, dim3(p.partial_rows), dim3(threads), 0, stream, b));
                 countLaunch();
                 return static_cast<int>(THOR_B200_OK);
             }

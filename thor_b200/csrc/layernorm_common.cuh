@@ -38,6 +38,28 @@ __device__ __forceinline__ float2 teamSum(float2 v, uint32_t team, uint32_t team
     const float other = __shfl_xor_sync(0xffffffffu, s, 16);
     return lane < 16 ? make_float2(s, other) : make_float2(other, s);
 }
+// The same for one row, or for two: four values, a quarter-warp keeps one each (teams of at most 384 threads).
+__device__ __forceinline__ void teamSums(float2 (&v)[1], uint32_t team, uint32_t team_id, Scratch& scratch, int slot) { v[0] = teamSum(v[0], team, team_id, scratch, slot); }
+__device__ __forceinline__ void teamSums(float2 (&v)[2], uint32_t team, uint32_t team_id, Scratch& scratch, int slot) {
+    constexpr uint32_t all = 0xffffffffu;
+    const uint32_t lane = threadIdx.x % 32, warps = team / 32, warp = threadIdx.x / 32 - team_id * warps;
+    const bool second = lane & 16, odd = lane & 8;  // which row, which of its values a lane keeps
+    float2 u = second ? v[1] : v[0];
+    const float2 give = second ? v[0] : v[1];
+    u = add2(u, make_float2(__shfl_xor_sync(all, give.x, 16), __shfl_xor_sync(all, give.y, 16)));
+    float s = odd ? u.y : u.x;
+    s += __shfl_xor_sync(all, odd ? u.x : u.y, 8);
+#pragma unroll
+    for (int o = 4; o > 0; o /= 2) s += __shfl_xor_sync(all, s, o);
+    float(*part)[4] = reinterpret_cast<float(*)[4]>(&scratch.part[slot][team_id][0]);  // [warp][value]: one team, or two of six warps
+    if (lane % 8 == 0) part[warp][lane / 8] = s;
+    asm volatile("bar.sync %0, %1;" ::"r"(team_id + 1), "r"(team) : "memory");
+    s = (lane % 8 < warps ? part[lane % 8][lane / 8] : 0.0f) + (lane % 8 + 8 < warps ? part[lane % 8 + 8][lane / 8] : 0.0f);
+#pragma unroll
+    for (int o = 4; o > 0; o /= 2) s += __shfl_xor_sync(all, s, o);
+    v[0] = make_float2(__shfl_sync(all, s, 0), __shfl_sync(all, s, 8));
+    v[1] = make_float2(__shfl_sync(all, s, 16), __shfl_sync(all, s, 24));
+}
 // Columns that a warp of a team holds, `chunks_a_thread` runs of 512 a team apart.
 __device__ __forceinline__ float warpColumns(uint32_t warp, uint32_t team, uint32_t cols, int chunks_a_thread) {
     uint32_t n = 0;
