@@ -115,6 +115,25 @@ def test_column_slices_and_leading_axes(dtype, first, cols, width):
     assert torch.equal(target, want)  # nothing beside the slice is written
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("cols,width", [(2033, 2049), (2047, 2047), (2048, 2065), (2049, 2096), (2064, 2081), (4097, 4097), (8193, 8195)])
+def test_long_odd_rows(dtype, code, cols, width):
+    """Rows that start at every place of 32 bytes in turn (odd widths), at one place (2096) and at every start of the first; each block has a magnitude
+    of its own, so that a code with a neighbour's scale shows; nothing beside the rows is written."""
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(35, cols, device="cuda", generator=gen)
+    x *= torch.exp2(torch.randint(-8, 8, (35, cols // 32 + 1), device="cuda", generator=gen).float()).repeat_interleave(32, 1)[:, :cols]
+    ck = CheckpointPack(from_torch(code)).stamp(x).run()
+    want = unpack64(ck.codes, ck.scales, cols).to(dtype)
+    for start in range(18):
+        buffer = torch.full((start + 35 * width + 40,), 7.0, device="cuda", dtype=dtype)
+        whole = buffer.clone()
+        CheckpointUnpack(from_torch(dtype)).stamp(ck, buffer.as_strided((35, cols), (width, 1), start)).run()
+        whole.as_strided((35, cols), (width, 1), start).copy_(want)
+        assert torch.equal(buffer, whole), start
+
+
 def test_a_range_of_rows_is_a_checkpoint():
     x = torch.randn(50, 70, device="cuda").bfloat16()
     whole = CheckpointPack().stamp(x).run()

@@ -63,6 +63,35 @@ def test_forward_and_backward(rows, cols, dtype, gated, kind):
         assert back.grad_gate is None
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("cols,width", [(2047, 2047), (2049, 2096), (4097, 4099), (2064, 2080)])
+def test_backward_of_long_odd_rows(dtype, kind, gated, cols, width):
+    """The same rows through tensors that all start at one place of 32 bytes, whichever it is, and through tensors that do not: the same bits, and
+    nothing beside the rows is written.  (Aligned tensors of the next width that 16 divides give the values to compare with.)"""
+    rows, padded = 19, (cols + 15) // 16 * 16
+    x, gate, grad = (torch.zeros(rows, padded, device="cuda", dtype=dtype) for _ in range(3))
+    for i, t in enumerate((x, gate, grad)):
+        t[:, :cols] = values(rows, cols, dtype, 30 + i) * torch.exp2(torch.arange(cols, device="cuda") // 32 % 5 - 2.0).to(dtype)
+    forward = CheckpointedActivation(KINDS[kind]).stamp(x, gate if gated else None)
+    forward.run()
+    plain = CheckpointedActivationBackward(KINDS[kind]).stamp(grad, forward.checkpoint, forward.gate_checkpoint)
+    plain.run()
+    kept = [ActivationCheckpoint(c.codes, c.scales, cols) if c is not None else None for c in (forward.checkpoint, forward.gate_checkpoint)]
+    starts = [(s, s, s) for s in range(17)] + [(3, 4, 3), (3, 3, 4), (0, 16, 5)]
+    for starts_of in starts:
+        buffers = [torch.full((s + rows * width + 40,), 7.0, device="cuda", dtype=dtype) for s in starts_of]
+        views = [b.as_strided((rows, cols), (width, 1), s) for b, s in zip(buffers, starts_of)]
+        views[0].copy_(grad[:, :cols])
+        CheckpointedActivationBackward(KINDS[kind]).stamp(views[0], *kept, grad_input=views[1], grad_gate=views[2] if gated else None).run()
+        for b, s, want in zip(buffers[1:], starts_of[1:], (plain.grad_input, plain.grad_gate)):
+            whole = torch.full_like(b, 7.0)
+            if want is not None:
+                whole.as_strided((rows, cols), (width, 1), s).copy_(want[:, :cols])
+            assert torch.equal(b, whole), starts_of
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_the_whole_range_of_the_function(kind):
     """From where the result underflows to where it is x itself, both signs; fp32 so that nothing is hidden by a rounding."""

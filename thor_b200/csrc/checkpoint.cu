@@ -32,6 +32,20 @@ __global__ void __launch_bounds__(kThreads) unpackKernel(Reader in, T* __restric
     store16<ALIGNED>(y + rowStart(row, y_stride) + col, col, cols, v, lane > 0 && col > 0, lane < 31);
 }
 
+// Odd rows of at least 2048 columns.
+template <class T>
+__global__ void __launch_bounds__(kThreads) unpackShiftedKernel(Reader in, T* __restrict__ y, uint32_t y_stride, uint32_t cols) {
+    gridDependencyWait();
+    gridLaunchDependents();
+    const uint32_t row = blockIdx.y;
+    T* const out = y + rowStart(row, y_stride);
+    const Place place = placeOf(out, cols);
+    if (place.first >= cols + place.m) return;
+    float2 v[8];
+    expandPlace(in.code, place, fetchPlace(in, place, row), v);
+    storePlace(place, out, v);
+}
+
 }  // namespace
 }  // namespace tb
 
@@ -84,6 +98,12 @@ int thor_b200_checkpoint_unpack_launch(const thor_b200_checkpoint_desc* d, const
     const bool aligned = rowsAligned(y, d->stride, d->dtype, d->rows) && d->cols % kVec == 0;
     return byDtype(d->dtype, [&](auto t) {
         using T = decltype(t);
+        if (!aligned && w.row_a_cta) {
+            shiftedGrid<T>(d->rows, d->cols, &grid, &block);
+            TB_CUDA(launchDependent(unpackShiftedKernel<T>, grid, block, 0, stream, in, static_cast<T*>(y), strideOf(d->stride, d->rows), static_cast<uint32_t>(d->cols)));
+            countLaunch();
+            return static_cast<int>(THOR_B200_OK);
+        }
         return byFlag(aligned, [&](auto a) {
             TB_CUDA(launchDependent(unpackKernel<T, decltype(a)::value>, grid, block, 0, stream, in, static_cast<T*>(y), strideOf(d->stride, d->rows), w));
             countLaunch();

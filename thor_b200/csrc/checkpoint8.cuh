@@ -127,15 +127,15 @@ __device__ __forceinline__ uint4 encode16(const float2 (&v)[8], uint32_t byte, i
 }
 
 template <int CODE>
-__device__ __forceinline__ void unpack4(uint32_t c, float2 s, float2& a, float2& b) {
+__device__ __forceinline__ void unpack4(uint32_t c, float2& a, float2& b) {
     if constexpr (CODE == THOR_B200_INT8) {
         // byte + 128 in the low bits of 2^23 is the float 2^23 + 128 + value; both steps are exact
         const uint32_t u = c ^ 0x80808080u;
         const float2 off = both(-8388736.0f);
         a = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)));
         b = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)));
-        a = mul2(add2(a, off), s);
-        b = mul2(add2(b, off), s);
+        a = add2(a, off);
+        b = add2(b, off);
     } else {
         uint32_t lo, hi;
         if constexpr (CODE == THOR_B200_FP8_E4M3) {
@@ -145,22 +145,28 @@ __device__ __forceinline__ void unpack4(uint32_t c, float2 s, float2& a, float2&
             lo = __byte_perm(c, 0u, 0x1404);
             hi = __byte_perm(c, 0u, 0x3424);
         }
-        a = mul2(__half22float2(*reinterpret_cast<const __half2*>(&lo)), s);
-        b = mul2(__half22float2(*reinterpret_cast<const __half2*>(&hi)), s);
+        a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+        b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     }
 }
 template <int CODE>
-__device__ __forceinline__ void decodeAs(uint4 c, float2 s, float2 (&v)[8]) {
-    unpack4<CODE>(c.x, s, v[0], v[1]);
-    unpack4<CODE>(c.y, s, v[2], v[3]);
-    unpack4<CODE>(c.z, s, v[4], v[5]);
-    unpack4<CODE>(c.w, s, v[6], v[7]);
+__device__ __forceinline__ void numbersAs(uint4 c, float2 (&v)[8]) {
+    unpack4<CODE>(c.x, v[0], v[1]);
+    unpack4<CODE>(c.y, v[2], v[3]);
+    unpack4<CODE>(c.z, v[4], v[5]);
+    unpack4<CODE>(c.w, v[6], v[7]);
+}
+// The numbers that codes stand for before they are scaled.
+__device__ __forceinline__ void numbers16(uint4 c, int code, float2 (&v)[8]) {
+    if (code == THOR_B200_FP8_E4M3) numbersAs<THOR_B200_FP8_E4M3>(c, v);
+    else if (code == THOR_B200_INT8) numbersAs<THOR_B200_INT8>(c, v);
+    else numbersAs<THOR_B200_FP8_E5M2>(c, v);
 }
 __device__ __forceinline__ void decode16(uint4 c, uint32_t byte, int code, float2 (&v)[8]) {
     const float2 s = both(scaleValue(byte));
-    if (code == THOR_B200_FP8_E4M3) decodeAs<THOR_B200_FP8_E4M3>(c, s, v);
-    else if (code == THOR_B200_INT8) decodeAs<THOR_B200_INT8>(c, s, v);
-    else decodeAs<THOR_B200_FP8_E5M2>(c, s, v);
+    numbers16(c, code, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], s);
 }
 
 // ---- sixteen neighbouring elements of a row ---------------------------------------------------------------
@@ -359,26 +365,25 @@ __device__ __forceinline__ void load16(const Rows<T>& in, const T* p, uint32_t c
     expand16(p, col, cols, raw, v);
 }
 
+__device__ __forceinline__ void store256(void* to, const uint32_t* w) {
+    asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
 // Writes sixteen values to columns col .. of a row of `cols`, from p on; a lane with cols = 0 writes nothing.  All 32 lanes call it.
 // Not ALIGNED: a lane writes the words of eight elements (32 bytes of fp32, 16 of a 16-bit type) that start in its range, the first of them with the
 // last elements of the lane before it; `before` / `after`: that lane / the lane behind holds the sixteen columns before / behind these.  Where a
 // neighbour is missing its part is left out, and what is left is written in smaller pieces; words that reach over the row's end are
-// written element by element.  (32-byte words of 16-bit types take twice the exchanges and cases: unpack [8192, 8191] bf16 46.6 us against 42;
-// 16-byte words of fp32 leave half a sector to every store: unpack [4096, 2999] 15.3 us against 9.5.)
+// written element by element.  (32-byte words of 16-bit types take twice the exchanges and cases: unpack [8192, 8191] bf16, when it stored its rows this way, 46.6 us
+// against 42; 16-byte words of fp32 leave half a sector to every store: unpack [4096, 2999] 15.3 us against 9.5.)
 template <bool ALIGNED, class T>
 __device__ __forceinline__ void store16(T* p, uint32_t col, uint32_t cols, const float2 (&v)[8], bool before, bool after) {
     constexpr int N = kRegs<T>;
     uint32_t own[N];
     narrow16<T>(v, own);
-    auto wide = [](void* to, const uint32_t* w) {
-        asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
-                     "r"(w[7])
-                     : "memory");
-    };
     if constexpr (ALIGNED) {
         if (col >= cols) return;
 #pragma unroll
-        for (int i = 0; i < N; i += 8) wide(reinterpret_cast<uint32_t*>(p) + i, own + i);
+        for (int i = 0; i < N; i += 8) store256(reinterpret_cast<uint32_t*>(p) + i, own + i);
     } else {
         constexpr int E = 8, PER = 4 / sizeof(T), W = E / PER;  // elements of a word, elements of a register, registers of a word
         uint32_t run[W + N];                                    // the lane before's last word and these
@@ -405,7 +410,7 @@ __device__ __forceinline__ void store16(T* p, uint32_t col, uint32_t cols, const
                     for (int e = 0; e < E; ++e)
                         if (first + e < left && (first + e >= 0 || before)) element(first + e, PER == 1 ? r[e % W] : r[e / 2] >> (16 * (e % 2)));
                 } else if (k > 0 || m == 0 || before) {
-                    if constexpr (W == 8) wide(p + first, r);
+                    if constexpr (W == 8) store256(p + first, r);
                     else __stcs(reinterpret_cast<uint4*>(p + first), make_uint4(r[0], r[1], r[2], r[3]));
                 } else {  // from element m of the word on
                     if constexpr (PER == 2 && m % 2 == 1) element(0, r[m / 2] >> 16);
@@ -489,10 +494,117 @@ __device__ __forceinline__ void expandCodes(int code, uint32_t col, uint32_t col
     if constexpr (CUT) cutRow(col, cols, v);
 }
 
+// ---- odd rows, walked on the tensor's own 32 bytes ---------------------------------------------------------
+// For kernels that read a checkpoint and write a tensor element by element: a thread takes the sixteen columns from 16 u - m on, m the elements by which
+// the row starts past 32 bytes, so that the tensor's words are whole and what has to be shifted are the codes, a quarter or an eighth of the bytes.
+// Elements before m come from the code word u - 1, the others from word u; m is the same for the whole CTA.
+// Against shifting the tensors' words: unpack [8192, 8191] bf16 42.0 -> 38.5 us, gated Swish backward 109.5 -> 95.9, GELU backward [8000, 5001] fp32 69.0 -> 55.9
+// and [2999, 11001] fp16 37.6 -> 35.8 ([8192, 8191] bf16 66.0 -> 69.8, the one that lost: a chunk more than two CTAs' threads a row).
+template <class T>
+constexpr uint32_t kShifts = 32 / sizeof(T);
+
+struct Place {
+    uint32_t first, m, cols;  // columns first - m ..
+    __device__ __forceinline__ bool whole() const { return first >= m && first - m + 16 <= cols; }
+    __device__ __forceinline__ bool holds(uint32_t i) const { return first + i >= m && first + i - m < cols; }
+};
+template <class T>
+__device__ __forceinline__ Place placeOf(const T* row, uint32_t cols) {
+    return Place{(blockIdx.x * blockDim.x + threadIdx.x) * kVec, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) / sizeof(T)) % kShifts<T>, cols};
+}
+template <class T>
+__device__ __forceinline__ T* at(const Place& q, T* row) {
+    return row + (static_cast<int64_t>(q.first) - q.m);
+}
+template <class T>
+__device__ __forceinline__ void loadPlace(const Place& q, const Rows<T>& in, const T* row, uint32_t (&w)[kRegs<T>]) {
+    const T* const p = at(q, row);
+    if (p >= in.p && static_cast<const void*>(p + 16) <= in.end) {  // what lies beside the row's columns is the tensor's, too, and not stored
+#pragma unroll
+        for (int i = 0; i < kRegs<T>; i += 8) {
+            uint4 lo, hi;
+            load256(lo, hi, reinterpret_cast<const uint32_t*>(p) + i);
+            w[i] = lo.x, w[i + 1] = lo.y, w[i + 2] = lo.z, w[i + 3] = lo.w;
+            w[i + 4] = hi.x, w[i + 5] = hi.y, w[i + 6] = hi.z, w[i + 7] = hi.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRegs<T>; i += 4) {
+            const uint4 u = edgeWord<T>(reinterpret_cast<const char*>(p) + 4 * i, in.p, in.end);
+            w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void storePlace(const Place& q, T* row, const float2 (&v)[8]) {
+    T* const p = at(q, row);
+    uint32_t w[kRegs<T>];
+    narrow16<T>(v, w);
+    if (q.whole()) {
+#pragma unroll
+        for (int i = 0; i < kRegs<T>; i += 8) store256(reinterpret_cast<uint32_t*>(p) + i, w + i);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (q.holds(i)) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool low = q.holds(2 * i), high = q.holds(2 * i + 1);
+            if (low && high) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+            else if (low) reinterpret_cast<uint16_t*>(p)[2 * i] = static_cast<uint16_t>(w[i]);
+            else if (high) reinterpret_cast<uint16_t*>(p)[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+        }
+    }
+}
+// The code words that a place needs and their scale bytes; m = 0 needs one.
+struct PlaceCodes {
+    uint4 a, b;
+    uint32_t scale_a, scale_b;
+};
+__device__ __forceinline__ PlaceCodes fetchPlace(const Reader& in, const Place& q, uint32_t row) {
+    PlaceCodes c{};
+    const uint8_t* const codes = codesAt(in, row, 0);
+    const uint8_t* const scales = scaleAt(in, row, 0);
+    if (q.first > 0 && q.m > 0) {
+        c.a = __ldg(reinterpret_cast<const uint4*>(codes + q.first) - 1);  // the neighbouring lane's, too: L1 keeps it
+        c.scale_a = __ldg(scales + (q.first - 16) / kBlock);
+    }
+    if (q.first < q.cols) {
+        c.b = __ldg(reinterpret_cast<const uint4*>(codes + q.first));
+        c.scale_b = __ldg(scales + q.first / kBlock);
+    }
+    return c;
+}
+__device__ __forceinline__ void expandPlace(int code, const Place& q, const PlaceCodes& c, float2 (&v)[8]) {
+    const uint32_t k = 16 - q.m;  // bytes of a that are left out
+    uint32_t r[8] = {c.a.x, c.a.y, c.a.z, c.a.w, c.b.x, c.b.y, c.b.z, c.b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = q.m == 0 ? r[i + 4] : r[i];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) r[i] = k & 8 ? r[i + 2] : r[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) r[i] = k & 4 ? r[i + 1] : r[i];
+    uint4 w;
+    w.x = __funnelshift_r(r[0], r[1], k % 4 * 8);
+    w.y = __funnelshift_r(r[1], r[2], k % 4 * 8);
+    w.z = __funnelshift_r(r[2], r[3], k % 4 * 8);
+    w.w = __funnelshift_r(r[3], r[4], k % 4 * 8);
+    numbers16(w, code, v);
+    const float a = scaleValue(c.scale_a), b = scaleValue(c.scale_b);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = mul2(v[i], make_float2(2 * i < q.m ? a : b, 2 * i + 1 < q.m ? a : b));
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------
 // Whether every row of a tensor starts on 32 bytes.
 inline bool rowsAligned(const void* p, int64_t stride, int dtype, uint64_t rows) {
     return p == nullptr || (isAligned(p, 32) && (rows <= 1 || (static_cast<uint64_t>(stride) * dtypeSize(dtype)) % 32 == 0));
+}
+// Whether two tensors' rows start at the same place of 32 bytes, all of them.
+inline bool rowsCongruent(const void* p, int64_t p_stride, const void* q, int64_t q_stride, int dtype) {
+    return (reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(q)) % 32 == 0 &&
+           (static_cast<uint64_t>(p_stride) - static_cast<uint64_t>(q_stride)) * dtypeSize(dtype) % 32 == 0;
 }
 // The stride of checked arguments; one row has none.
 inline uint32_t strideOf(int64_t stride, uint64_t rows) { return rows > 1 ? static_cast<uint32_t>(stride) : 0u; }

@@ -3,7 +3,7 @@
 // One chunk of sixteen columns per thread and one wave of CTAs after another: each thread has all its loads in flight before it uses the first.  A
 // tensor whose rows lie dense and whose width is a multiple of 32 is walked as one row; other rows of at least 2048 columns get CTAs of their
 // own (blockIdx.y is the row: no index division, addresses the same for the whole CTA; Swish backward [8192, 8191] bf16 66.8 -> 59.9 us),
-// shorter ones share CTAs.
+// which kernels that only read a checkpoint use to walk odd rows on the tensor's own 32 bytes; shorter ones share CTAs.
 #pragma once
 
 #include "checkpoint8.cuh"
@@ -42,6 +42,18 @@ __device__ __forceinline__ void locate(const Walk& w, uint32_t& row, uint32_t& c
     }
 }
 
+// A CTA for every row, or several where the row is longer than its threads take.
+inline void rowGrid(uint64_t rows, uint32_t chunks, dim3* grid, dim3* block) {
+    const uint32_t segments = (chunks + kThreads - 1) / kThreads;
+    *grid = dim3(segments, static_cast<unsigned>(rows));
+    *block = dim3(((chunks + segments - 1) / segments + 31) / 32 * 32);
+}
+// The same for odd rows that are walked on the tensor's own 32 bytes.
+template <class T>
+void shiftedGrid(uint64_t rows, uint64_t cols, dim3* grid, dim3* block) {
+    rowGrid(rows, static_cast<uint32_t>((cols + kShifts<T> - 1 + kVec - 1) / kVec), grid, block);
+}
+
 inline int planWalk(uint64_t rows, uint64_t cols, bool dense, Walk* w, dim3* grid, dim3* block) {
     if (dense && cols % kBlock == 0 && rows * cols < 0x80000000ull) {  // the checkpoint's rows are dense then, too
         cols *= rows;
@@ -52,9 +64,7 @@ inline int planWalk(uint64_t rows, uint64_t cols, bool dense, Walk* w, dim3* gri
     w->units = rows * w->chunks;
     w->row_a_cta = rows > 1 && rows <= 65535 && w->chunks >= 128;
     if (w->row_a_cta) {
-        const uint32_t segments = (w->chunks + kThreads - 1) / kThreads;
-        *grid = dim3(segments, static_cast<unsigned>(rows));
-        *block = dim3(((w->chunks + segments - 1) / segments + 31) / 32 * 32);
+        rowGrid(rows, w->chunks, grid, block);
         return THOR_B200_OK;
     }
     const uint64_t ctas = (w->units + kThreads - 1) / kThreads;

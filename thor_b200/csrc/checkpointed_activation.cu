@@ -135,6 +135,40 @@ __global__ void __launch_bounds__(kThreads, residentCtas<T, GATED, ALIGNED, true
     store16<ALIGNED>(grad_x + rowStart(row, grad_x_stride) + col, col, cols, dx, before, after);
 }
 
+// Odd rows of at least 2048 columns whose tensors all start at the same place of 32 bytes.  (Columns beside the row's may be loaded; they are not stored.)
+template <class T, int KIND, bool GATED>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : GATED ? 5 : 6) activationBackwardShiftedKernel(Rows<T> grad, Reader in, Reader gate_in, T* __restrict__ grad_x,
+                                                                     uint32_t grad_x_stride, T* __restrict__ grad_gate, uint32_t grad_gate_stride, uint32_t cols) {
+    gridDependencyWait();
+    gridLaunchDependents();
+    const uint32_t row = blockIdx.y;
+    const T* const grad_row = grad.p + rowStart(row, grad.stride);
+    const Place place = placeOf(grad_row, cols);
+    if (place.first >= cols + place.m) return;
+    uint32_t raw[kRegs<T>];
+    PlaceCodes gate_codes;
+    loadPlace(place, grad, grad_row, raw);
+    const PlaceCodes codes = fetchPlace(in, place, row);
+    if constexpr (GATED) gate_codes = fetchPlace(gate_in, place, row);
+    float2 d[8], v[8], dx[8];
+    expandPlace(in.code, place, codes, v);
+    widen16<T>(raw, d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float2 value, slope;
+        activation2<KIND, sizeof(T) == 4>(v[i], value, slope);
+        dx[i] = mul2(d[i], slope);
+        d[i] = mul2(d[i], value);
+    }
+    if constexpr (GATED) {
+        storePlace(place, grad_gate + rowStart(row, grad_gate_stride), d);
+        expandPlace(gate_in.code, place, gate_codes, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dx[i] = mul2(dx[i], v[i]);
+    }
+    storePlace(place, grad_x + rowStart(row, grad_x_stride), dx);
+}
+
 int checkActivation(const char* who, const thor_b200_checkpointed_activation_desc* d) {
     TB_REQUIRE(d != nullptr, "%s: null description", who);
     TB_REQUIRE(d->kind == THOR_B200_ACTIVATION_GELU || d->kind == THOR_B200_ACTIVATION_SWISH, "%s: unknown activation %d", who, d->kind);
@@ -215,8 +249,20 @@ int thor_b200_checkpointed_activation_backward_launch(const thor_b200_checkpoint
     bool aligned = false;
     if (int st = planActivation(*d, grad_input, grad_gate, grad_output, &w, &grid, &block, &aligned)) return st;
     const Reader in = readerOf(codes, scales, w.cols, d->code_dtype), gate_in = readerOf(gate_codes, gate_scales, w.cols, d->code_dtype);
+    const bool shifted = !aligned && w.row_a_cta && rowsCongruent(grad_output, d->y_stride, grad_input, d->x_stride, d->dtype) &&
+                         (!d->gated || rowsCongruent(grad_output, d->y_stride, grad_gate, d->gate_stride, d->dtype));
     return byVariant(*d, aligned, [&](auto t, auto kind, auto gated, auto a) {
         using T = decltype(t);
+        if constexpr (!decltype(a)::value) {
+            if (shifted) {
+                shiftedGrid<T>(d->rows, d->cols, &grid, &block);
+                TB_CUDA(launchDependent(activationBackwardShiftedKernel<T, decltype(kind)::value, decltype(gated)::value>, grid, block, 0, static_cast<cudaStream_t>(stream_v),
+                                        rowsOf<T>(grad_output, d->y_stride, d->rows, d->cols), in, gate_in, static_cast<T*>(grad_input), strideOf(d->x_stride, d->rows),
+                                        static_cast<T*>(grad_gate), strideOf(d->gate_stride, d->rows), static_cast<uint32_t>(d->cols)));
+                countLaunch();
+                return static_cast<int>(THOR_B200_OK);
+            }
+        }
         TB_CUDA(launchDependent(activationBackwardKernel<T, decltype(kind)::value, decltype(gated)::value, decltype(a)::value>, grid, block, 0,
                                 static_cast<cudaStream_t>(stream_v), rowsOf<T>(grad_output, d->y_stride, d->rows, d->cols), in, gate_in, static_cast<T*>(grad_input),
                                 strideOf(d->x_stride, d->rows), static_cast<T*>(grad_gate), strideOf(d->gate_stride, d->rows), w));
