@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kThreads) unpackShiftedKernel(Reader in, T* __
     const Place place = placeOf(out, cols);
     if (place.first >= cols + place.m) return;
     float2 v[8];
-    expandPlace(in.code, place, fetchPlace(in, place, row), v);
+    expandPlace<T, true>(in.code, place, fetchPlace(in, place, row), v);
     storePlace(place, out, v);
 }
 

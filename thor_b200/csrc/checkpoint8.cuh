@@ -498,8 +498,8 @@ __device__ __forceinline__ void expandCodes(int code, uint32_t col, uint32_t col
 // For kernels that read a checkpoint and write a tensor element by element: a thread takes the sixteen columns from 16 u - m on, m the elements by which
 // the row starts past 32 bytes, so that the tensor's words are whole and what has to be shifted are the codes, a quarter or an eighth of the bytes.
 // Elements before m come from the code word u - 1, the others from word u; m is the same for the whole CTA.
-// Against shifting the tensors' words: unpack [8192, 8191] bf16 42.0 -> 38.5 us, gated Swish backward 109.5 -> 95.9, GELU backward [8000, 5001] fp32 69.0 -> 55.9
-// and [2999, 11001] fp16 37.6 -> 35.8 ([8192, 8191] bf16 66.0 -> 69.8, the one that lost: a chunk more than two CTAs' threads a row).
+// Against shifting the tensors' words: unpack [8192, 8191] bf16 42.0 -> 34.8 us, gated Swish backward 109.5 -> 89.8, GELU backward 66.0 -> 60.8, [2999, 11001]
+// fp16 37.6 -> 31.1 and [8000, 5001] fp32 69.0 -> 54.0.
 template <class T>
 constexpr uint32_t kShifts = 32 / sizeof(T);
 
@@ -576,24 +576,52 @@ __device__ __forceinline__ PlaceCodes fetchPlace(const Reader& in, const Place& 
     }
     return c;
 }
+// Calls f with m as an integral constant below N; the whole CTA takes one branch.
+template <int N, class F>
+__device__ __forceinline__ void byConstant(uint32_t m, F&& f) {
+    if constexpr (N == 1) {
+        f(std::integral_constant<int, 0>{});
+    } else {
+        if (m < N / 2) byConstant<N / 2>(m, f);
+        else byConstant<N - N / 2>(m - N / 2, [&](auto i) { f(std::integral_constant<int, decltype(i)::value + N / 2>{}); });
+    }
+}
+// The sixteen values of a place.  Which byte goes where and which scale it takes hang on m alone: constants in each of the branches.  ONCE: the
+// branches hold the conversion of the codes, too (48 of them); otherwise only the shift and, once more, the scaling.  Once is the faster form (GELU backward
+// [8192, 8191] bf16 60.8 us against 67.3; with selects by m instead of branches 69.7), except in 16-bit gated kernels, whose two expansions
+// of 48 branches end up in local memory (220 us against 90).
+template <class T, bool ONCE>
 __device__ __forceinline__ void expandPlace(int code, const Place& q, const PlaceCodes& c, float2 (&v)[8]) {
-    const uint32_t k = 16 - q.m;  // bytes of a that are left out
-    uint32_t r[8] = {c.a.x, c.a.y, c.a.z, c.a.w, c.b.x, c.b.y, c.b.z, c.b.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = q.m == 0 ? r[i + 4] : r[i];
-#pragma unroll
-    for (int i = 0; i < 6; ++i) r[i] = k & 8 ? r[i + 2] : r[i];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) r[i] = k & 4 ? r[i + 1] : r[i];
-    uint4 w;
-    w.x = __funnelshift_r(r[0], r[1], k % 4 * 8);
-    w.y = __funnelshift_r(r[1], r[2], k % 4 * 8);
-    w.z = __funnelshift_r(r[2], r[3], k % 4 * 8);
-    w.w = __funnelshift_r(r[3], r[4], k % 4 * 8);
-    numbers16(w, code, v);
+    const uint32_t r[8] = {c.a.x, c.a.y, c.a.z, c.a.w, c.b.x, c.b.y, c.b.z, c.b.w};
     const float a = scaleValue(c.scale_a), b = scaleValue(c.scale_b);
+    auto shifted = [&](auto shift) {
+        constexpr int k = 16 - decltype(shift)::value;  // bytes of the first word that are left out
+        uint32_t w[4];
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) v[i] = mul2(v[i], make_float2(2 * i < q.m ? a : b, 2 * i + 1 < q.m ? a : b));
+        for (int i = 0; i < 4; ++i) w[i] = k % 4 == 0 ? r[k / 4 + i] : __funnelshift_r(r[k / 4 + i], r[(k / 4 + i + 1) % 8], k % 4 * 8);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto scale = [&](auto shift) {
+        constexpr int m = decltype(shift)::value;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], make_float2(2 * i < m ? a : b, 2 * i + 1 < m ? a : b));
+    };
+    if constexpr (ONCE) {
+        auto convert = [&](auto dtype) {
+            byConstant<kShifts<T>>(q.m, [&](auto shift) {
+                numbersAs<decltype(dtype)::value>(shifted(shift), v);
+                scale(shift);
+            });
+        };
+        if (code == THOR_B200_FP8_E4M3) convert(std::integral_constant<int, THOR_B200_FP8_E4M3>{});
+        else if (code == THOR_B200_INT8) convert(std::integral_constant<int, THOR_B200_INT8>{});
+        else convert(std::integral_constant<int, THOR_B200_FP8_E5M2>{});
+    } else {
+        uint4 w;
+        byConstant<kShifts<T>>(q.m, [&](auto shift) { w = shifted(shift); });
+        numbers16(w, code, v);
+        byConstant<kShifts<T>>(q.m, scale);
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------

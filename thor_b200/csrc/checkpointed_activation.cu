@@ -145,13 +145,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : GATED ? 5 : 6) 
     const T* const grad_row = grad.p + rowStart(row, grad.stride);
     const Place place = placeOf(grad_row, cols);
     if (place.first >= cols + place.m) return;
+    constexpr bool ONCE = !GATED || sizeof(T) == 4;
     uint32_t raw[kRegs<T>];
     PlaceCodes gate_codes;
     loadPlace(place, grad, grad_row, raw);
     const PlaceCodes codes = fetchPlace(in, place, row);
     if constexpr (GATED) gate_codes = fetchPlace(gate_in, place, row);
     float2 d[8], v[8], dx[8];
-    expandPlace(in.code, place, codes, v);
+    expandPlace<T, ONCE>(in.code, place, codes, v);
     widen16<T>(raw, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : GATED ? 5 : 6) 
     }
     if constexpr (GATED) {
         storePlace(place, grad_gate + rowStart(row, grad_gate_stride), d);
-        expandPlace(gate_in.code, place, gate_codes, v);
+        expandPlace<T, ONCE>(gate_in.code, place, gate_codes, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dx[i] = mul2(dx[i], v[i]);
     }
