@@ -309,14 +309,27 @@ __device__ __forceinline__ uint32_t wordAt(const uint32_t (&r)[N], int e) {
     else return e % 2 == 0 ? r[e / 2] : __funnelshift_r(r[e / 2], r[e / 2 + 1], 16);
 }
 
-// Zeroes the columns past the row's end.
+// Calls f with m as an integral constant below N; where m is the same for a whole warp it takes one branch.
+template <int N, class F>
+__device__ __forceinline__ void byConstant(uint32_t m, F&& f) {
+    if constexpr (N == 1) {
+        f(std::integral_constant<int, 0>{});
+    } else {
+        if (m < N / 2) byConstant<N / 2>(m, f);
+        else byConstant<N - N / 2>(m - N / 2, [&](auto i) { f(std::integral_constant<int, decltype(i)::value + N / 2>{}); });
+    }
+}
+// Zeroes the columns past the row's end, in the lane that holds it; its place is the same in every row, so by constants (LayerNorm forward [20000, 333] bf16
+// 16.5 -> 14.5 us against comparing each column).
 __device__ __forceinline__ void cutRow(uint32_t col, uint32_t cols, float2 (&v)[8]) {
-    if (col + 16 > cols) {
+    if (col < cols && col + 16 > cols) {
+        byConstant<16>(cols - col, [&](auto n) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (col + 2 * i >= cols) v[i].x = 0.0f;
-            if (col + 2 * i + 1 >= cols) v[i].y = 0.0f;
-        }
+            for (int i = 0; i < 8; ++i) {
+                if (2 * i >= decltype(n)::value) v[i].x = 0.0f;
+                if (2 * i + 1 >= decltype(n)::value) v[i].y = 0.0f;
+            }
+        });
     }
 }
 
@@ -575,16 +588,6 @@ __device__ __forceinline__ PlaceCodes fetchPlace(const Reader& in, const Place& 
         c.scale_b = __ldg(scales + q.first / kBlock);
     }
     return c;
-}
-// Calls f with m as an integral constant below N; the whole CTA takes one branch.
-template <int N, class F>
-__device__ __forceinline__ void byConstant(uint32_t m, F&& f) {
-    if constexpr (N == 1) {
-        f(std::integral_constant<int, 0>{});
-    } else {
-        if (m < N / 2) byConstant<N / 2>(m, f);
-        else byConstant<N - N / 2>(m - N / 2, [&](auto i) { f(std::integral_constant<int, decltype(i)::value + N / 2>{}); });
-    }
 }
 // The sixteen values of a place.  Which byte goes where and which scale it takes hang on m alone: constants in each of the branches.  ONCE: the
 // branches hold the conversion of the codes, too (48 of them); otherwise only the shift and, once more, the scaling.  Once is the faster form (GELU backward
