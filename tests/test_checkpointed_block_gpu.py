@@ -8,7 +8,7 @@ import torch
 from _layers64 import activation64, layernorm_grads64, unpack64
 from thor_b200 import DataType, _native
 from thor_b200.activation import CheckpointedActivation, CheckpointedActivationBackward, CheckpointedActivationKind as Kind
-from thor_b200.checkpoint import CheckpointPack, CheckpointUnpack
+from thor_b200.checkpoint import ActivationCheckpoint, CheckpointPack, CheckpointUnpack
 from thor_b200.normalization import LayerNorm, LayerNormBackward
 
 pytestmark = pytest.mark.gpu
@@ -125,3 +125,35 @@ def test_kept_tensor_between_steps_of_other_sizes():
     Block(torch.bfloat16, DataType.fp8_e4m3, Kind.Swish).step()
     for ck, want in kept:
         assert torch.equal(CheckpointUnpack(DataType.fp32).stamp(ck).run(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(5, 33), (9, 2049), (600, 1001), (3, 8193)])
+def test_padding_is_not_read_and_a_broken_block_stays_a_block(dtype, rows, cols):
+    """Whatever bytes lie in a checkpoint's padding, results are the same; a block whose scale is NaN gives NaN in its own columns only."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x, grad = (torch.randn(rows, cols, device="cuda", generator=gen).to(dtype) for _ in range(2))
+    gamma, rstd = 1 + 0.1 * torch.randn(cols, device="cuda", generator=gen), 1 + torch.rand(rows, device="cuda", generator=gen)
+    for code in (DataType.fp8_e4m3, DataType.int8):
+        clean = CheckpointPack(code).stamp(x).run()
+        dirty = ActivationCheckpoint(clean.codes.clone(), clean.scales.clone(), cols)
+        dirty.codes.view(torch.uint8)[:, cols:] = 0x7F  # NaN in e4m3, 127 in int8
+        results = []
+        for ck in (clean, dirty):
+            norm = LayerNormBackward().stamp(grad, rstd, gamma=gamma, checkpoint=ck)
+            act = CheckpointedActivationBackward(Kind.Gelu).stamp(grad, ck, ck)
+            results.append([CheckpointUnpack(DataType.fp32).stamp(ck).run(), norm.run(), norm.grad_gamma, norm.grad_beta, act.run(), act.grad_gate])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+        block = (cols - 1) // 32 // 2
+        dirty.scales.view(torch.uint8)[rows // 2, block] = 255
+        broken = torch.zeros(rows, cols, dtype=torch.bool, device="cuda")
+        broken[rows // 2, 32 * block:32 * block + 32] = True
+        act = CheckpointedActivationBackward(Kind.Gelu).stamp(grad, dirty, dirty)
+        act.run()
+        for got, want in ((CheckpointUnpack(DataType.fp32).stamp(dirty).run(), results[0][0]), (act.grad_input, results[0][4]), (act.grad_gate, results[0][5])):
+            assert torch.equal(torch.isnan(got), broken) and torch.equal(got[~broken], want[~broken])
+        norm = LayerNormBackward().stamp(grad, rstd, gamma=gamma, checkpoint=dirty)
+        got = norm.run()
+        others = torch.arange(rows, device="cuda") != rows // 2
+        assert torch.isnan(got[rows // 2]).all() and torch.equal(got[others], results[0][1][others])
+        assert torch.equal(torch.isnan(norm.grad_gamma), broken[rows // 2]) and torch.equal(norm.grad_beta, results[0][3])
