@@ -41,7 +41,7 @@ class StampedCheckpointedActivation(Stamped):
         self.output, self.checkpoint, self.gate_checkpoint = output, checkpoint, gate_checkpoint
         desc = _ActivationDesc(int(kind), int(gate is not None), int(from_torch(x.dtype)), int(checkpoint.dtype), rows, cols, x_stride, gate_stride, y_stride)
         super().__init__(_lib.thor_b200_checkpointed_activation_launch,
-                         (C.byref(desc), x.data_ptr(), gate.data_ptr() if gate is not None else None, output.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(),
+                         (C.addressof(desc), x.data_ptr(), gate.data_ptr() if gate is not None else None, output.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(),
                           gate_checkpoint.codes.data_ptr() if gate is not None else None, gate_checkpoint.scales.data_ptr() if gate is not None else None),
                          x.device, stream, (x, gate, desc))
 
@@ -82,7 +82,7 @@ class StampedCheckpointedActivationBackward(Stamped):
         self.grad_input, self.grad_gate = grad_input, grad_gate
         desc = _ActivationDesc(int(kind), int(gated), int(from_torch(grad_output.dtype)), int(checkpoint.dtype), rows, cols, x_stride, gate_stride, y_stride)
         super().__init__(_lib.thor_b200_checkpointed_activation_backward_launch,
-                         (C.byref(desc), grad_output.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(),
+                         (C.addressof(desc), grad_output.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(),
                           gate_checkpoint.codes.data_ptr() if gated else None, gate_checkpoint.scales.data_ptr() if gated else None,
                           grad_input.data_ptr(), grad_gate.data_ptr() if gated else None), grad_output.device, stream, (grad_output, checkpoint, gate_checkpoint, desc))
 

@@ -54,7 +54,7 @@ class StampedLayerNorm(Stamped):
     def __init__(self, desc, x, gamma, beta, residual, output, total, mean, rstd, checkpoint, stream):
         self.output, self.sum, self.mean, self.rstd, self.checkpoint = output, total, mean, rstd, checkpoint
         super().__init__(_lib.thor_b200_layernorm_launch,
-                         (C.byref(desc), _ptr(x), _ptr(residual), _ptr(gamma), _ptr(beta), _ptr(output), _ptr(total), _ptr(mean), _ptr(rstd),
+                         (C.addressof(desc), _ptr(x), _ptr(residual), _ptr(gamma), _ptr(beta), _ptr(output), _ptr(total), _ptr(mean), _ptr(rstd),
                           _ptr(checkpoint.codes) if checkpoint is not None else None, _ptr(checkpoint.scales) if checkpoint is not None else None),
                          x.device, stream, (x, gamma, beta, residual, desc))
 
@@ -106,7 +106,7 @@ class StampedLayerNormBackward(Stamped):
         self.grad_gamma, self.grad_beta = (grad_params[0], grad_params[1]) if grad_params is not None else (None, None)
         self.kernel_launches = int(_lib.thor_b200_layernorm_backward_launch_count(C.byref(desc), int(grad_params is not None)))
         super().__init__(_lib.thor_b200_layernorm_backward_launch,
-                         (C.byref(desc), _ptr(grad_output), _ptr(x), _ptr(mean), _ptr(rstd), _ptr(checkpoint.codes) if checkpoint is not None else None,
+                         (C.addressof(desc), _ptr(grad_output), _ptr(x), _ptr(mean), _ptr(rstd), _ptr(checkpoint.codes) if checkpoint is not None else None,
                           _ptr(checkpoint.scales) if checkpoint is not None else None, _ptr(gamma), _ptr(grad_sum), _ptr(grad_input), _ptr(self.grad_gamma), _ptr(self.grad_beta),
                           _ptr(workspace), workspace.numel() if workspace is not None else 0),
                          grad_output.device, stream, (grad_output, rstd, gamma, x, mean, checkpoint, grad_sum, workspace, desc))
