@@ -93,7 +93,8 @@ class StampedCheckpointedActivationBackward(Stamped):
 
 class CheckpointedActivationBackward:
     """grad_input = grad_output * act'(x) with x from its checkpoint; with the gate's checkpoint too, grad_input = grad_output * gate * act'(x)
-    and grad_gate = grad_output * act(x).  The gradients may be column slices of one buffer."""
+    and grad_gate = grad_output * act(x).  The gradients may be column slices of one buffer.  Where x was masked with its type's lowest number, whose
+    code stands for 2^128, both gradients are zero."""
 
     def __init__(self, kind: CheckpointedActivationKind):
         self.kind = CheckpointedActivationKind(kind)

@@ -89,8 +89,13 @@ __device__ __forceinline__ uint32_t scaleByte(float amax, int code) {
     const int byte = max(static_cast<int>((bits + carry) >> 23) - exponent, 0);
     return bits >= 0x7f800000u ? 255u : static_cast<uint32_t>(byte);
 }
+// FINITE, for gradients: a magnitude within half a step of 2^128 (a type's lowest number, as masks write it) has the code of 2^128, an infinity in fp32, and an
+// infinity times a slope or a gradient of zero would be NaN.  Scales that reach so far (from 2^113 on) are one unit in the last place smaller there, so
+// that 2^128 becomes the largest number.
+template <bool FINITE = false>
 __device__ __forceinline__ float scaleValue(uint32_t byte) {
-    return __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255u ? 0x7fc00000u : byte << 23));
+    const uint32_t power = FINITE ? (byte << 23) - (byte >= 240u ? 1u : 0u) : byte << 23;
+    return __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255u ? 0x7fc00000u : power));
 }
 
 template <int CODE>
@@ -162,8 +167,9 @@ __device__ __forceinline__ void numbers16(uint4 c, int code, float2 (&v)[8]) {
     else if (code == THOR_B200_INT8) numbersAs<THOR_B200_INT8>(c, v);
     else numbersAs<THOR_B200_FP8_E5M2>(c, v);
 }
+template <bool FINITE>
 __device__ __forceinline__ void decode16(uint4 c, uint32_t byte, int code, float2 (&v)[8]) {
-    const float2 s = both(scaleValue(byte));
+    const float2 s = both(scaleValue<FINITE>(byte));
     numbers16(c, code, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], s);
@@ -501,9 +507,9 @@ __device__ __forceinline__ void fetchCodes(const uint8_t* codes, const uint8_t* 
     raw.scale = __ldg(scale);
 }
 // CUT: the padding behind the row's end is made zero whatever the block's scale.
-template <bool CUT>
+template <bool CUT, bool FINITE = false>
 __device__ __forceinline__ void expandCodes(int code, uint32_t col, uint32_t cols, const RawCodes& raw, float2 (&v)[8]) {
-    decode16(raw.codes, raw.scale, code, v);
+    decode16<FINITE>(raw.codes, raw.scale, code, v);
     if constexpr (CUT) cutRow(col, cols, v);
 }
 
@@ -593,10 +599,10 @@ __device__ __forceinline__ PlaceCodes fetchPlace(const Reader& in, const Place& 
 // branches hold the conversion of the codes, too (48 of them); otherwise only the shift and, once more, the scaling.  Once is the faster form (GELU backward
 // [8192, 8191] bf16 60.8 us against 67.3; with selects by m instead of branches 69.7), except in 16-bit gated kernels, whose two expansions
 // of 48 branches end up in local memory (220 us against 90).
-template <class T, bool ONCE>
+template <class T, bool ONCE, bool FINITE = false>
 __device__ __forceinline__ void expandPlace(int code, const Place& q, const PlaceCodes& c, float2 (&v)[8]) {
     const uint32_t r[8] = {c.a.x, c.a.y, c.a.z, c.a.w, c.b.x, c.b.y, c.b.z, c.b.w};
-    const float a = scaleValue(c.scale_a), b = scaleValue(c.scale_b);
+    const float a = scaleValue<FINITE>(c.scale_a), b = scaleValue<FINITE>(c.scale_b);
     auto shifted = [&](auto shift) {
         constexpr int k = 16 - decltype(shift)::value;  // bytes of the first word that are left out
         uint32_t w[4];

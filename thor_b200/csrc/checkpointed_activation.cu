@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, residentCtas<T, GATED, ALIGNED, true
     fetchCodes(codesAt(in, row, col), scaleAt(in, row, col), col, cols, codes);
     if constexpr (GATED) fetchCodes(codesAt(gate_in, row, col), scaleAt(gate_in, row, col), col, cols, gate_codes);
     float2 d[8], v[8], dx[8];
-    expandCodes<false>(in.code, col, cols, codes, v);  // columns past the row's end are not stored
+    expandCodes<false, true>(in.code, col, cols, codes, v);  // columns past the row's end are not stored
     expand16(grad_at, col, cols, raw, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, residentCtas<T, GATED, ALIGNED, true
     const bool before = lane > 0 && col > 0, after = lane < 31;
     if constexpr (GATED) {
         store16<ALIGNED>(grad_gate + rowStart(row, grad_gate_stride) + col, col, cols, d, before, after);
-        expandCodes<false>(gate_in.code, col, cols, gate_codes, v);
+        expandCodes<false, true>(gate_in.code, col, cols, gate_codes, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dx[i] = mul2(dx[i], v[i]);
     }
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : GATED ? 5 : 6) 
     const PlaceCodes codes = fetchPlace(in, place, row);
     if constexpr (GATED) gate_codes = fetchPlace(gate_in, place, row);
     float2 d[8], v[8], dx[8];
-    expandPlace<T, ONCE>(in.code, place, codes, v);
+    expandPlace<T, ONCE, true>(in.code, place, codes, v);
     widen16<T>(raw, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : GATED ? 5 : 6) 
     }
     if constexpr (GATED) {
         storePlace(place, grad_gate + rowStart(row, grad_gate_stride), d);
-        expandPlace<T, ONCE>(gate_in.code, place, gate_codes, v);
+        expandPlace<T, ONCE, true>(gate_in.code, place, gate_codes, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dx[i] = mul2(dx[i], v[i]);
     }
