@@ -43,7 +43,7 @@ class StampedCheckpointedActivation(Stamped):
         super().__init__(_lib.thor_b200_checkpointed_activation_launch,
                          (C.addressof(desc), x.data_ptr(), gate.data_ptr() if gate is not None else None, output.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(),
                           gate_checkpoint.codes.data_ptr() if gate is not None else None, gate_checkpoint.scales.data_ptr() if gate is not None else None),
-                         x.device, stream, (x, gate, desc))
+                         x.device, stream, (x, gate, output, checkpoint, gate_checkpoint, desc))
 
     def run(self) -> torch.Tensor:
         self._call()
@@ -84,7 +84,8 @@ class StampedCheckpointedActivationBackward(Stamped):
         super().__init__(_lib.thor_b200_checkpointed_activation_backward_launch,
                          (C.addressof(desc), grad_output.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(),
                           gate_checkpoint.codes.data_ptr() if gated else None, gate_checkpoint.scales.data_ptr() if gated else None,
-                          grad_input.data_ptr(), grad_gate.data_ptr() if gated else None), grad_output.device, stream, (grad_output, checkpoint, gate_checkpoint, desc))
+                          grad_input.data_ptr(), grad_gate.data_ptr() if gated else None), grad_output.device, stream,
+                         (grad_output, checkpoint, gate_checkpoint, grad_input, grad_gate, desc))
 
     def run(self) -> torch.Tensor:
         self._call()

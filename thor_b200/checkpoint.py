@@ -103,15 +103,16 @@ def check_outputs(outputs: dict, inputs: dict) -> None:
 
 
 class Stamped:
-    """What the stamped operators share: run() is one call of `launch` with arguments resolved at stamp time (integers;
-    the description by its address, kept alive in `keep`) and the stream of the moment."""
+    """What the stamped operators share: run() is one call of `launch` with arguments resolved at stamp time (integers: the addresses of the
+    description and of tensors, all of which `keep` keeps alive, outputs and the tensors of checkpoints among them) and the stream of the moment."""
 
     def __init__(self, launch, args: tuple, device: torch.device, stream, keep: tuple):
         # a function object of its own that takes every argument as a pointer-sized integer: the description's pointer type and the conversions cost 0.3 us a call
         self._launch = _lib[launch.__name__]
         self._launch.argtypes = [C.c_void_p] * (len(args) + 1)
         self._args, self._device = args, device.index if device.index is not None else torch.cuda.current_device()
-        self._stream, self._keep = stream, keep
+        self._stream = stream
+        self._keep = [(k.codes, k.scales) if isinstance(k, ActivationCheckpoint) else k for k in keep]
         if stream is not None and stream.device.index != self._device:
             refuse("the stream must belong to the tensors' device")
 
@@ -201,7 +202,8 @@ class StampedCheckpointPack(Stamped):
         check_outputs({"codes": checkpoint.codes, "scales": checkpoint.scales}, {"the tensor": x})
         self.checkpoint = checkpoint
         desc = _CheckpointDesc(int(from_torch(x.dtype)), int(checkpoint.dtype), rows, cols, stride)
-        super().__init__(_lib.thor_b200_checkpoint_pack_launch, (C.addressof(desc), x.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr()), x.device, stream, (x, desc))
+        super().__init__(_lib.thor_b200_checkpoint_pack_launch, (C.addressof(desc), x.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr()), x.device, stream,
+                         (x, checkpoint, desc))
 
     def run(self) -> ActivationCheckpoint:
         self._call()
@@ -227,7 +229,7 @@ class StampedCheckpointUnpack(Stamped):
         self.checkpoint, self.output = checkpoint, output
         desc = _CheckpointDesc(int(from_torch(output.dtype)), int(checkpoint.dtype), rows, cols, stride)
         super().__init__(_lib.thor_b200_checkpoint_unpack_launch, (C.addressof(desc), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(), output.data_ptr()), output.device, stream,
-                         (desc,))
+                         (checkpoint, output, desc))
 
     def run(self) -> torch.Tensor:
         self._call()

@@ -56,7 +56,7 @@ class StampedLayerNorm(Stamped):
         super().__init__(_lib.thor_b200_layernorm_launch,
                          (C.addressof(desc), _ptr(x), _ptr(residual), _ptr(gamma), _ptr(beta), _ptr(output), _ptr(total), _ptr(mean), _ptr(rstd),
                           _ptr(checkpoint.codes) if checkpoint is not None else None, _ptr(checkpoint.scales) if checkpoint is not None else None),
-                         x.device, stream, (x, gamma, beta, residual, desc))
+                         x.device, stream, (x, gamma, beta, residual, output, total, mean, rstd, checkpoint, desc))
 
     def run(self) -> torch.Tensor:
         self._call()
@@ -109,7 +109,7 @@ class StampedLayerNormBackward(Stamped):
                          (C.addressof(desc), _ptr(grad_output), _ptr(x), _ptr(mean), _ptr(rstd), _ptr(checkpoint.codes) if checkpoint is not None else None,
                           _ptr(checkpoint.scales) if checkpoint is not None else None, _ptr(gamma), _ptr(grad_sum), _ptr(grad_input), _ptr(self.grad_gamma), _ptr(self.grad_beta),
                           _ptr(workspace), workspace.numel() if workspace is not None else 0),
-                         grad_output.device, stream, (grad_output, rstd, gamma, x, mean, checkpoint, grad_sum, workspace, desc))
+                         grad_output.device, stream, (grad_output, rstd, gamma, x, mean, checkpoint, grad_sum, grad_input, grad_params, workspace, desc))
 
     def run(self) -> torch.Tensor:
         self._call()
