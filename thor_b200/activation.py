@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from .checkpoint import ActivationCheckpoint, Stamped, as_rows, check_outputs, code_dtype, matching_checkpoint, refuse, same_rows, target_checkpoint
+from .checkpoint import ActivationCheckpoint, Stamped, as_rows, check_outputs, code_dtype, matching_checkpoint, memory_of, refuse, same_rows, target_checkpoint
 from .dtypes import DataType, from_torch
 
 _lib = _native.lib
@@ -61,11 +61,12 @@ class CheckpointedActivation:
         rows, cols, _ = as_rows(x, "CheckpointedActivation: x")
         if gate is None and gate_checkpoint is not None:
             refuse("CheckpointedActivation: gate_checkpoint without a gate")
-        if output is None:
-            output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        checkpoint = target_checkpoint(checkpoint, rows, cols, self.checkpoint_dtype, x.device, "CheckpointedActivation: checkpoint")
-        if gate is not None:
-            gate_checkpoint = target_checkpoint(gate_checkpoint, rows, cols, self.checkpoint_dtype, x.device, "CheckpointedActivation: gate_checkpoint")
+        with memory_of(stream):
+            if output is None:
+                output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            checkpoint = target_checkpoint(checkpoint, rows, cols, self.checkpoint_dtype, x.device, "CheckpointedActivation: checkpoint")
+            if gate is not None:
+                gate_checkpoint = target_checkpoint(gate_checkpoint, rows, cols, self.checkpoint_dtype, x.device, "CheckpointedActivation: gate_checkpoint")
         return StampedCheckpointedActivation(self.kind, x, gate, output, checkpoint, gate_checkpoint, stream)
 
 
@@ -110,8 +111,9 @@ class CheckpointedActivationBackward:
                 refuse("CheckpointedActivationBackward: both checkpoints must hold the same code dtype")
         elif grad_gate is not None:
             refuse("CheckpointedActivationBackward: grad_gate without the gate's checkpoint")
-        if grad_input is None:
-            grad_input = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
-        if gate_checkpoint is not None and grad_gate is None:
-            grad_gate = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
+        with memory_of(stream):
+            if grad_input is None:
+                grad_input = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
+            if gate_checkpoint is not None and grad_gate is None:
+                grad_gate = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
         return StampedCheckpointedActivationBackward(self.kind, grad_output, checkpoint, gate_checkpoint, grad_input, grad_gate, stream)

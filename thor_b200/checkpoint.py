@@ -2,10 +2,12 @@
 
 An operator is described once, stamped on its tensors (checks, output allocation) and run as often as the step repeats; run()
 is one call into the library on the stream given at stamp time or, without one, on the current stream, and allocates nothing, so it can be
-captured into a CUDA graph.  A stamped operator owns its outputs and workspace: two runs of one plan (direct or as replays of graphs that hold
+captured into a CUDA graph.  A stamped operator owns its outputs and workspace, which belong to the stream given at stamp time or, without one, to the
+one that was current then (a run on another stream is ordered behind that one by the caller, as for any tensor): two runs of one plan (direct or as replays of graphs that hold
 it) must not overlap in time, and a plan must outlive the work and the graphs that use it; plans of the same operator are independent of one another."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional
 
@@ -100,6 +102,11 @@ def check_outputs(outputs: dict, inputs: dict) -> None:
         for other, u in out[i + 1:] + [(n, u) for n, u in inputs.items() if u is not None]:
             if t.device == u.device and not _disjoint(t, u):
                 refuse(f"{name} overlaps {other}")
+
+
+def memory_of(stream):
+    """Context in which a plan allocates what it owns: memory of the stream that it will run on, so that nothing still pending on another one uses it."""
+    return torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
 
 
 class Stamped:
@@ -218,7 +225,9 @@ class CheckpointPack:
 
     def stamp(self, x: torch.Tensor, checkpoint: Optional[ActivationCheckpoint] = None, stream=None) -> StampedCheckpointPack:
         rows, cols, _ = as_rows(x, "CheckpointPack: the tensor")
-        return StampedCheckpointPack(x, target_checkpoint(checkpoint, rows, cols, self.dtype, x.device, "CheckpointPack: checkpoint"), stream)
+        with memory_of(stream):
+            checkpoint = target_checkpoint(checkpoint, rows, cols, self.dtype, x.device, "CheckpointPack: checkpoint")
+        return StampedCheckpointPack(x, checkpoint, stream)
 
 
 class StampedCheckpointUnpack(Stamped):
@@ -250,7 +259,8 @@ class CheckpointUnpack:
         if not isinstance(checkpoint, ActivationCheckpoint):
             refuse("CheckpointUnpack: needs an ActivationCheckpoint")
         if output is None:
-            output = torch.empty(checkpoint.rows, checkpoint.cols, dtype=to_torch(self.dtype), device=checkpoint.device)
+            with memory_of(stream):
+                output = torch.empty(checkpoint.rows, checkpoint.cols, dtype=to_torch(self.dtype), device=checkpoint.device)
         elif output.dtype != to_torch(self.dtype):
             refuse(f"CheckpointUnpack: output must be {self.dtype.name}")
         return StampedCheckpointUnpack(checkpoint, output, stream)

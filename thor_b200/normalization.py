@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from .checkpoint import ActivationCheckpoint, Stamped, VALUE_DTYPES, as_rows, check_outputs, code_dtype, matching_checkpoint, refuse, same_rows, target_checkpoint
+from .checkpoint import ActivationCheckpoint, Stamped, VALUE_DTYPES, as_rows, check_outputs, code_dtype, matching_checkpoint, memory_of, refuse, same_rows, target_checkpoint
 from .dtypes import DataType, from_torch, to_torch
 
 _lib = _native.lib
@@ -81,17 +81,18 @@ class LayerNorm:
         rows, cols, x_stride = as_rows(x, "LayerNorm: x")
         residual_stride = same_rows(residual, "LayerNorm: residual", x) if residual is not None else 0
         param = _check_params("LayerNorm", x, gamma=gamma, beta=beta)
-        if output is None:
-            output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        y_stride = same_rows(output, "LayerNorm: output", x)
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
         if checkpoint is not None and self.checkpoint_dtype is None:
             refuse("LayerNorm: described without a checkpoint")
-        if self.checkpoint_dtype is not None:
-            checkpoint = target_checkpoint(checkpoint, rows, cols, self.checkpoint_dtype, x.device, "LayerNorm: checkpoint")
-        statistic = lambda: torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        rstd = statistic() if self.save_statistics else None
-        mean = statistic() if self.save_statistics and checkpoint is None else None
+        with memory_of(stream):
+            if output is None:
+                output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+            if self.checkpoint_dtype is not None:
+                checkpoint = target_checkpoint(checkpoint, rows, cols, self.checkpoint_dtype, x.device, "LayerNorm: checkpoint")
+            statistic = lambda: torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+            rstd = statistic() if self.save_statistics else None
+            mean = statistic() if self.save_statistics and checkpoint is None else None
+        y_stride = same_rows(output, "LayerNorm: output", x)
         check_outputs({"output": output, "codes": checkpoint.codes if checkpoint else None, "scales": checkpoint.scales if checkpoint else None},
                       {"x": x, "residual": residual, "gamma": gamma, "beta": beta})
         desc = _LayerNormDesc(int(from_torch(x.dtype)), int(param), 0, int(self.checkpoint_dtype or 0), self.eps, 0, rows, cols, x_stride, residual_stride, y_stride)
@@ -145,13 +146,15 @@ class LayerNormBackward:
         sum_stride = same_rows(grad_sum, f"{who}: grad_sum", grad_output) if grad_sum is not None else 0
         param = _check_params(who, grad_output, gamma=gamma)
         grad_param = self.grad_dtype if self.grad_dtype is not None else param
-        grad_input = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=device)
-        grad_params = torch.empty(2, cols, dtype=to_torch(grad_param), device=device) if gamma is not None else None
+        with memory_of(stream):
+            grad_input = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=device)
+            grad_params = torch.empty(2, cols, dtype=to_torch(grad_param), device=device) if gamma is not None else None
         desc = _LayerNormDesc(int(from_torch(grad_output.dtype)), int(param), int(grad_param), int(checkpoint.dtype) if checkpoint is not None else 0, 0.0, 0, rows, cols, x_stride,
                               sum_stride, y_stride)
         workspace = None
         if gamma is not None:
             size = C.c_size_t()
             _native.check(_lib.thor_b200_layernorm_backward_workspace_bytes(C.byref(desc), C.byref(size)))
-            workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+            with memory_of(stream):
+                workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
         return StampedLayerNormBackward(desc, grad_output, rstd, gamma, x, mean, checkpoint, grad_sum, grad_input, grad_params, workspace, stream)
