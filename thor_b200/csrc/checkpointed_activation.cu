@@ -32,6 +32,13 @@ __device__ __forceinline__ void activation2(float2 x, float2& value, float2& slo
         const float2 s = make_float2(right_x ? r.x : er.x, right_y ? r.y : er.y), rest = make_float2(right_x ? er.x : r.x, right_y ? er.y : r.y);
         value = mul2(x, s);
         slope = fma2(value, rest, s);
+    } else if constexpr (KIND == THOR_B200_ACTIVATION_SWISH && std::is_same<T, __nv_bfloat16>::value) {
+        // The reciprocal of 2^-16 (1 + 2^y): of 1 + 2^y it would be zero below 2^-126, left of x = -87.3.  fp16 has no results so small.
+        const float2 y = fma2(x, both(-1.44269504f), both(-16.0f)), low = both(1.52587890625e-5f);
+        const float2 d = add2(make_float2(exp2Approx(y.x), exp2Approx(y.y)), low);
+        const float2 s = mul2(make_float2(reciprocalApprox(d.x), reciprocalApprox(d.y)), low);
+        value = mul2(x, s);
+        slope = fma2(value, fma2(s, both(-1.0f), both(1.0f)), s);
     } else if constexpr (KIND == THOR_B200_ACTIVATION_SWISH) {
         const float2 y = mul2(x, both(-1.44269504f));
         const float2 d = add2(make_float2(exp2Approx(y.x), exp2Approx(y.y)), both(1.0f));
