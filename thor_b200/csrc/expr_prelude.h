@@ -85,20 +85,18 @@ __device__ __forceinline__ __half2 tb_bits2half2(unsigned int v) {
     *reinterpret_cast<unsigned int*>(&r) = v;
     return r;
 }
-// exp(x) = 2^(x log2 e).  For a result that is normal in fp16 |t| = |x log2 e| <= 16, so the rounded product is off by at most
-// 2^-21 and the rounded constant by 16 * 1.4e-8 of an exponent, and ex2.approx by 2^-22 of its result: together below 7.5e-7,
-// 13 units of the 24-bit result.  fp16 drops 13 of those bits, so the rounding is certain unless they lie within 13 units of the
-// midpoint 2^12 (0.33 % of the results) or the result is subnormal in fp16, where more bits are dropped.
+// exp(x) = 2^(x log2 e), with Ziv's test: what lies 1.3e-6 of the value above and below it is rounded, too, and where the two agree so does the
+// exponential.  A result above zero in fp16 has |t| = |x log2 e| <= 25, so the product's rounding (2^-20 of an exponent) and the constant's (25 * 1.4e-8) cost at most
+// 9.0e-7 of the result, ex2.approx 2^-22 and the two products here 6e-8: 1.2e-6 together.  (0.3 % of the results fail.  Comparing the
+// dropped bits with their midpoint and testing for subnormal results apart took three times the instructions.)
 __device__ __forceinline__ __half2 tb_h2exp(const __half2 a) {
-    const float2 f = __half22float2(a);
-    float lo, hi;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(f.x * 1.44269504f));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(f.y * 1.44269504f));
-    const __half2 r = __floats2half2_rn(lo, hi);
-    const unsigned int bits = *reinterpret_cast<const unsigned int*>(&r);
-    const bool near_midpoint = ((__float_as_uint(lo) - (0x1000u - 13u)) & 0x1FFFu) <= 26u || ((__float_as_uint(hi) - (0x1000u - 13u)) & 0x1FFFu) <= 26u;
-    const bool subnormal = ((bits & 0xFFFFu) - 1u) < 0x3FFu || ((bits >> 16) - 1u) < 0x3FFu;
-    if (near_midpoint || subnormal) return h2exp(a);
+    const float2 t = __fmul2_rn(__half22float2(a), make_float2(1.44269504f, 1.44269504f));
+    float2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    const float2 above = __fmul2_rn(e, make_float2(1.0000013f, 1.0000013f)), below = __fmul2_rn(e, make_float2(0.9999987f, 0.9999987f));
+    const __half2 r = __floats2half2_rn(above.x, above.y), s = __floats2half2_rn(below.x, below.y);
+    if (*reinterpret_cast<const unsigned int*>(&r) != *reinterpret_cast<const unsigned int*>(&s)) return h2exp(a);
     return r;
 }
 // Argument known to be <= 0 (or NaN).
@@ -124,8 +122,9 @@ __device__ __forceinline__ __half2 tb_h2div(const __half2 a, const __half2 b) {
     const __half2 v = __floats2half2_rn(rx * fa.x, ry * fa.y);
     // A quotient of two 11-bit significands is never the midpoint of two normal fp16 numbers (midpoint * divisor would need
     // more than the dividend's 11 bits), but it can be the midpoint of two subnormal ones, where the product's error decides.
+    // A lane is subnormal if bits + 0x7c00 does not reach its top bit and bits + 0x7fff does (it is not zero); neither sum leaves its lane.
     const unsigned int bits = *reinterpret_cast<const unsigned int*>(&v) & 0x7fff7fffu;
-    if (((bits & 0xffffu) - 1u) < 0x3FFu || ((bits >> 16) - 1u) < 0x3FFu) return __h2div(a, b);
+    if (~(bits + 0x7c007c00u) & (bits + 0x7fff7fffu) & 0x80008000u) return __h2div(a, b);
     return v;
 }
 
