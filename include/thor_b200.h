@@ -214,7 +214,7 @@ THOR_B200_API size_t thor_b200_jit_cache_size(void);
 /* 16-bit stages evaluate exp and division with leaner routines than cuda_fp16.hpp's h2exp / __h2div, the
  * intrinsics the reference emits (CudaSourceEmitter.cpp:4376-4377).  This self-check runs both over every fp16
  * input (exp) and every ordered input pair in both lanes (division) and writes four counters to device
- * memory: [0] exp mismatches, [1] mismatches of the variant used for arguments known to be <= 0, [2] division
+ * memory: [0] exp mismatches, [1] exp mismatches over a second pattern of lanes (arguments <= 0 or NaN), [2] division
  * mismatches, [3] division pairs checked (2^32).  Bit parity with the reference requires [0..2] == 0. */
 THOR_B200_API int thor_b200_selfcheck_pair_math(unsigned long long* device_counters, void* stream);
 

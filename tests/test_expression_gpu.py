@@ -205,7 +205,7 @@ def test_run_rejects_multi_stage_expressions():
 
 
 def test_lean_pair_math_is_bit_identical_to_the_toolkit_intrinsics():
-    """tb_h2exp / tb_h2exp_nonpos / tb_h2div against h2exp / __h2div: all 65536 inputs, all 2^32 pairs, both lanes."""
+    """tb_h2exp / tb_h2div against h2exp / __h2div: all 65536 inputs, all 2^32 pairs, both lanes."""
     import ctypes as C
 
     import torch

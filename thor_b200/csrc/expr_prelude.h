@@ -99,8 +99,6 @@ __device__ __forceinline__ __half2 tb_h2exp(const __half2 a) {
     if (*reinterpret_cast<const unsigned int*>(&r) != *reinterpret_cast<const unsigned int*>(&s)) return h2exp(a);
     return r;
 }
-// Argument known to be <= 0 (or NaN).
-__device__ __forceinline__ __half2 tb_h2exp_nonpos(const __half2 a) { return tb_h2exp(a); }
 // Lane-wise z < 0 ? if_negative : otherwise (false for -0 and NaN, like the comparison).
 __device__ __forceinline__ __half2 tb_h2sel_neg(const __half2 z, const __half2 if_negative, const __half2 otherwise) {
     const unsigned int m = __hlt2_mask(z, __half2half2(__ushort_as_half((unsigned short)0)));
