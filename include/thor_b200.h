@@ -502,7 +502,7 @@ THOR_B200_API int thor_b200_checkpoint_unpack_launch(const thor_b200_checkpoint_
  *                                                               grad_gate  = grad_output * act(x~)
  *             (a code that stands for 2^128 is the largest fp32 number here: a place masked with the type's lowest number has gradients of zero)
  * gelu(x) = x * normcdf(x), swish(x) = x * sigmoid(x), as in Expression::gelu / Expression::swish.  Computed in fp32, one
- * rounding.  x_stride / gate_stride / y_stride are the row strides of x, gate and y and, in the backward pass, of grad_input,
+ * rounding; gelu' comes as zero left of x = -13.2, where it is below 6e-38.  x_stride / gate_stride / y_stride are the row strides of x, gate and y and, in the backward pass, of grad_input,
  * grad_gate and grad_output: the two halves of one [rows, 2 * cols] projection and of its gradient need no copy. */
 enum { THOR_B200_ACTIVATION_GELU = 0, THOR_B200_ACTIVATION_SWISH = 1 };
 

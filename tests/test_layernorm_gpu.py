@@ -1,5 +1,5 @@
-"""LayerNorm forward and backward against the 64-bit definition, at the lengths where the kernels change (groups of lanes up to 1024 columns,
-a CTA's registers up to 32768, loops above).
+"""LayerNorm forward and backward against the 64-bit definition, at lengths on both sides of those where the kernels change (a group of lanes up to 512
+columns, whole warps above; loops above 16384 columns forward, 8192 backward).
 
 Bounds.  A sum of n fp32 values in any order whose longest chain of additions is D has error at most D 2^-24 sum|v|; every sum here is taken
 per thread, per row group and (column sums) per slab in turn, with D below 512 for the shapes tested."""

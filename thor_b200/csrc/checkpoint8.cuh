@@ -2,8 +2,9 @@
 //
 // A block is 32 neighbouring columns of one row.  Its scale is the smallest power of two s with max|x| <= s * M, M the
 // largest code (448 for e4m3, 57344 for e5m2, 127 for int8), stored as the byte log2(s) + 127 (e8m0); a code is x / s
-// rounded to nearest even.  Division and multiplication by a power of two are exact, so a value that is packed again from its
-// own unpacked form gives the same code, and pack / unpack have exactly one rounding.  s is clamped at 2^-127 from below (an
+// rounded to nearest even.  Division and multiplication by a power of two are exact, so pack / unpack have exactly one rounding, and a block that is
+// packed again from its own unpacked form stands for the same values (maybe by other codes: 450 packs as 224 with s = 2, and the 448 it unpacks to as 448
+// with s = 1).  s is clamped at 2^-127 from below (an
 // all-zero block has that scale).  A block that holds an infinity or a NaN has the scale byte 255 and codes zero, and
 // unpacks as NaN throughout: an overflow stays visible in the backward pass.
 //
@@ -293,8 +294,10 @@ __device__ __forceinline__ void fetch16(const Rows<T>& in, const T* p, uint32_t 
     }
 }
 
-// Calls f with m as an integral constant, m elements past a word of eight elements.  Every row has one m, so a warp takes one or two of the branches,
-// and each of them moves whole registers (and shifts pairs by half a register where m is odd) instead of selecting by m.
+// Calls f with m as an integral constant, m elements past a word of eight elements.  Every row has one m, so a warp of one or two rows takes one or two of the
+// branches, and each of them moves whole registers (and shifts pairs by half a register where m is odd) instead of selecting by m.  Rows of fewer than 256 columns put 3 to
+// 16 rows into a warp, which then takes up to eight branches: bf16 [1000000, 33] pack 44 us, unpack 89, GELU 126 each way, LayerNorm 147 and 174, 0.15 to 0.35 of the
+// copy rate; [262144, 97] 0.28 to 0.55; [60000, 333] 0.32 to 0.67.
 template <class T, class F>
 __device__ __forceinline__ void byOffset(const void* p, F&& f) {
     switch ((static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) / sizeof(T)) % 8) {

@@ -87,8 +87,8 @@ __device__ __forceinline__ __half2 tb_bits2half2(unsigned int v) {
 }
 // exp(x) = 2^(x log2 e), with Ziv's test: what lies 1.3e-6 of the value above and below it is rounded, too, and where the two agree so does the
 // exponential.  A result above zero in fp16 has |t| = |x log2 e| <= 25, so the product's rounding (2^-20 of an exponent) and the constant's (25 * 1.4e-8) cost at most
-// 9.0e-7 of the result, ex2.approx 2^-22 and the two products here 6e-8: 1.2e-6 together.  (0.3 % of the results fail.  Comparing the
-// dropped bits with their midpoint and testing for subnormal results apart took three times the instructions.)
+// 9.0e-7 of the result, ex2.approx 2^-22 and the two products here 6e-8: 1.2e-6 together.  0.3 % of the results fail, which sends one warp in six to the toolkit.
+// (Comparing the dropped bits with their midpoint and testing for subnormal results apart took three times the instructions.)
 __device__ __forceinline__ __half2 tb_h2exp(const __half2 a) {
     const float2 t = __fmul2_rn(__half22float2(a), make_float2(1.44269504f, 1.44269504f));
     float2 e;

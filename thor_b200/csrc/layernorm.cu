@@ -16,7 +16,8 @@ using namespace ln;
 constexpr uint64_t kRegisterCols = 512ull * 2 * kVec;  // longest row of a team's registers: 512 threads, two chunks each
 
 // CTAs of 512 threads an SM holds: one chunk a thread needs 64 registers, two need 128.  Up to 8192 columns one chunk is the faster form (more warps
-// to wait with): [32768, 8192] bf16 with checkpoint 230 us against 255 with two and 80 registers and 334 with two and 128.
+// to wait with): [32768, 8192] bf16 with checkpoint, in runs of a few milliseconds, 230 us against 255 with two and 80 registers and 334 with two and 128 (at
+// sustained clocks the first takes 250).
 constexpr int residentCtas(int chunks) { return chunks == 1 ? 2 : 1; }
 
 template <class T>
