@@ -17,8 +17,10 @@ using namespace ck8;
 // Phi(-|x|) = e^(-x^2/2) R(|x|), where R(a) = erfcx(a / sqrt 2) / 2 is smooth and falls from 1/2 like 0.4 / a: R is a polynomial in
 // t = 1 / (1 + p a) without a constant term, fitted here for the least relative error over 0 <= a <= 15, past which the
 // exponential is below the smallest normal number.  The form keeps the relative accuracy of the far tail, and the exponential is the one
-// that the derivative needs.  Degree 9: 2.1e-7 of the value as evaluated in fp32 (fp32 tensors); degree 6: 4.8e-6, a hundredth of
-// half a unit of fp16 (16-bit tensors), three instructions a pair less.  For fp32 the rounding of x^2 is carried into the exponent.
+// that the derivative needs.  Degree 9: 2.1e-7 of R as evaluated in fp32 (fp32 tensors); degree 6: 4.8e-6, a hundredth of
+// half a unit of fp16 (16-bit tensors), three instructions a pair less.  For fp32 what the exponent's roundings lose is carried into the exponential: gelu is off by at
+// most 8 units of 2^-24 of itself, by 66 where the exponent keeps its own rounding ([8192, 8192] 89 -> 90 us forward, 142 -> 145 gated backward; [8192, 8191] 102 -> 108
+// forward, 101 -> 105 and, gated, 142 -> 160 backward).
 // Two elements an instruction (f32x2) and one exponential and one reciprocal an element; with the toolkit's erfcf and expf the backward kernel
 // waited for the arithmetic pipes.
 template <class T, int KIND>
@@ -66,14 +68,20 @@ __device__ __forceinline__ void activation2(float2 x, float2& value, float2& slo
             r = fma2(r, t, both(0.12044038f));
             r = fma2(r, t, both(0.12386077f));
         }
-        const float2 square = mul2(x, x);
-        const float2 half_log2e = both(-0.72134752f);
-        float2 y = mul2(square, half_log2e);
-        if constexpr (FULL) {  // square and its rounding error; an infinite x has no error to carry
-            const float2 lost = fma2(x, x, make_float2(-square.x, -square.y));
-            y = fma2(square, half_log2e, mul2(make_float2(a.x < 1e18f ? lost.x : 0.0f, a.y < 1e18f ? lost.y : 0.0f), half_log2e));
+        float2 e;
+        if constexpr (FULL) {
+            // y = -square log2(e) / 2 and what it lacks: its own rounding, that of the constant, and what square lost.  Past 32 nothing is left of e.
+            const float2 c = make_float2(fminf(a.x, 32.0f), fminf(a.y, 32.0f)), square = mul2(c, c), n = mul2(square, both(0.72134752f));
+            const float2 lost = fma2(c, c, make_float2(-square.x, -square.y));
+            float2 low = fma2(square, both(-0.72134752f), n);
+            low = fma2(lost, both(-0.72134752f), low);
+            low = fma2(square, both(-9.629814956e-9f), low);
+            e = make_float2(exp2Approx(-n.x), exp2Approx(-n.y));
+            e = fma2(mul2(e, both(0.69314718f)), low, e);
+        } else {
+            const float2 y = mul2(mul2(x, x), both(-0.72134752f));
+            e = make_float2(exp2Approx(y.x), exp2Approx(y.y));
         }
-        const float2 e = make_float2(exp2Approx(y.x), exp2Approx(y.y));
         const float2 rt = mul2(r, t);
         const float2 q = mul2(rt, e), p = mul2(fma2(a, both(-0.39894228f), rt), e);  // Phi and slope at -|x|; those at x and -x add up to one
         const float2 phi = make_float2(x.x > 0.0f ? 1.0f - q.x : q.x, x.y > 0.0f ? 1.0f - q.y : q.y);
